@@ -18,6 +18,7 @@ import random
 
 import numpy as np
 import torch
+import torch.utils.dlpack
 
 own = False  # run() computes plain forms; true: it calls the framework's operators
 
@@ -205,7 +206,7 @@ def _handles(s, c):
     def hold(t):
         x = B.zeros(t.numel())
         B.synchronize()
-        torch.as_tensor(x, device="cuda").copy_(t.reshape(-1))
+        torch.from_dlpack(x).copy_(t.reshape(-1))
         torch.cuda.synchronize()
         return x
 
@@ -232,7 +233,8 @@ def run(s):
 
 
 def _view(x, *shape):
-    return torch.as_tensor(x, device="cuda").view(*shape)
+    # the storage itself: whoever reads the outputs waits for the device first
+    return torch.utils.dlpack.from_dlpack(x.__dlpack__(stream=-1)).view(*shape)
 
 
 def _own_rope(s, c):
