@@ -5,7 +5,7 @@ include/scry_hip.h); this package is the host-side mirror of the reference
 interface: ``HipBackend`` (backend trait methods), ``LlamaModel`` /
 ``LlamaKvCache`` / ``generate`` (llama.rs, kv_cache.rs, generate.rs).
 """
-from .backend import HipBackend, I8Storage, Storage, init  # noqa: F401
+from .backend import HipBackend, I8Storage, KvCache8, Storage, init  # noqa: F401
 from .linear import Linear, QuantState, normal_vec  # noqa: F401
 from .llama import (QUANT_BF16, QUANT_BLOCK32, QUANT_PER_TENSOR, LlamaConfig, LlamaKvCache,  # noqa: F401
                     LlamaModel, Rng, SamplingConfig, bench_qgemv, generate)

@@ -111,6 +111,17 @@ SIGNATURES = {
     "scry_hip_split_qkv_reshape_heads": [vp, i32, i32, i32, P(vp), P(vp), P(vp)],
     "scry_hip_reshape_for_heads": [vp, i32, i32, i32, i32, P(vp)],
     "scry_hip_reshape_from_heads": [vp, i32, i32, i32, i32, P(vp)],
+    "scry_hip_buf_dlpack": [vp, vp, i32, P(vp)],
+    "scry_hip_qk_norm_rope": [vp, i32, i32, vp, vp, i32, i32, i32, vp, vp, vp, f32, f32, P(vp), P(vp), P(vp)],
+    "scry_hip_kv8_new": [i32, i32, i32, P(vp)],
+    "scry_hip_kv8_free": [vp],
+    "scry_hip_kv8_write": [vp, i32, vp, i32, vp, vp],
+    "scry_hip_kv8_read": [vp, i32, vp, i32, P(vp), P(vp)],
+    "scry_hip_kv8_keep": [vp, i32, vp, vp, i32],
+    "scry_hip_tree_attention": [vp, vp, vp, i32, vp, i32, vp, i32, i32, i32, f32, P(vp)],
+    "scry_hip_kv8_tree_attention": [vp, vp, i32, vp, i32, vp, i32, f32, P(vp)],
+    "scry_hip_verify_draft": [vp, vp, vp, vp, vp, i32, i32, i32, vp, vp],
+    "scry_hip_verify_tree": [vp, vp, vp, vp, i32, i32, i32, vp, vp, vp],
     "scry_hip_llama_new_random": [P(LlamaConfigC), u64, i32, i32, P(vp)],
     "scry_hip_llama_from_safetensors": [P(LlamaConfigC), P(C.c_char_p), i32, i32, P(vp)],
     "scry_hip_llama_free": [vp],

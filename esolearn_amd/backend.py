@@ -15,6 +15,25 @@ from . import _lib
 from ._lib import call, load
 
 
+_CAPSULE_NEW = C.pythonapi.PyCapsule_New
+_CAPSULE_NEW.restype, _CAPSULE_NEW.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
+C.pythonapi.PyCapsule_IsValid.argtypes = [C.c_void_p, C.c_char_p]
+C.pythonapi.PyCapsule_GetPointer.restype = C.c_void_p
+C.pythonapi.PyCapsule_GetPointer.argtypes = [C.c_void_p, C.c_char_p]
+
+
+@C.PYFUNCTYPE(None, C.c_void_p)
+def _capsule_end(capsule):
+    """A capsule that nobody took (who takes one renames it) ends its view."""
+    if C.pythonapi.PyCapsule_IsValid(capsule, b"dltensor"):
+        m = C.pythonapi.PyCapsule_GetPointer(capsule, b"dltensor")
+        deleter = C.cast(m + 56, C.POINTER(C.CFUNCTYPE(None, C.c_void_p)))[0]  # after the tensor (48 bytes) and the context
+        deleter(m)
+
+
+_CAPSULE_END = C.cast(_capsule_end, C.c_void_p)
+
+
 def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32).ravel()
 
@@ -32,6 +51,20 @@ class Storage:
         out = np.empty(self.n, np.float32)
         call("scry_hip_to_vec", self.h, out.ctypes.data, self.n)
         return out
+
+    def __dlpack_device__(self) -> tuple[int, int]:
+        return 10, 0  # ROCm; the library runs on one device (init)
+
+    def __dlpack__(self, stream=None, **_):
+        """The f32 values where they lie on the device, without a copy, for
+        torch.from_dlpack and its like (torch imported before this package, so
+        that both use one HIP runtime).  stream: what it does next comes after
+        the ops called so far (None, 0, 1: the default stream); -1: the caller
+        waits, as with HipBackend.synchronize().  Writes through the view, and
+        reads that outlive it, are ordered by the caller."""
+        m = C.c_void_p()
+        call("scry_hip_buf_dlpack", self.h, None if stream in (None, 0, 1, -1) else stream, int(stream != -1), C.byref(m))
+        return _CAPSULE_NEW(m, b"dltensor", _CAPSULE_END)
 
     def free(self) -> None:
         if self.h:
@@ -71,8 +104,67 @@ class I8Storage:
             pass
 
 
+class KvCache8:
+    """An int8 KV cache of max_seq rows of one layer and one sequence."""
+
+    __slots__ = ("h", "max_seq", "n_kv", "head_dim")
+
+    def __init__(self, handle: int, max_seq: int, n_kv: int, head_dim: int):
+        self.h = handle
+        self.max_seq = max_seq
+        self.n_kv = n_kv
+        self.head_dim = head_dim
+
+    def free(self) -> None:
+        if self.h:
+            load().scry_hip_kv8_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 def _out():
     return C.c_void_p()
+
+
+def _ints(a, dtype=np.int32) -> np.ndarray:
+    """A host array of whole numbers, refused where dtype does not hold them."""
+    x = np.ascontiguousarray(a)
+    if x.dtype != dtype:
+        y = x.astype(dtype)
+        if not np.array_equal(x, y):
+            raise ValueError(f"expected values that {np.dtype(dtype).name} holds")
+        x = y
+    return x
+
+
+def _starts(start) -> np.ndarray:
+    a = _ints(start)
+    if a.ndim != 1:
+        raise ValueError("one context length per sequence")
+    return a
+
+
+def _parents(parents, n_seq: int, rows: int):
+    """[n_seq, rows] parents, or one tree [rows] that every sequence has."""
+    if parents is None:
+        return None, None
+    a = _ints(parents)
+    if a.shape == (rows,):
+        a = np.ascontiguousarray(np.broadcast_to(a, (n_seq, rows)))
+    if a.shape != (n_seq, rows):
+        raise ValueError(f"parents must be [{n_seq}, {rows}] or [{rows}]")
+    return a, a.ctypes.data
+
+
+def _handles(items, n_seq: int):
+    if len(items) != n_seq:
+        raise ValueError("one cache per sequence")
+    return (C.c_void_p * n_seq)(*[i.h for i in items])
 
 
 def _st(h: C.c_void_p, n: int) -> Storage:
@@ -438,9 +530,121 @@ class HipBackend:
         call("scry_hip_reshape_from_heads", x.h, batch, seq, n_heads, d_head, C.byref(o))
         return _st(o, batch * seq * n_heads * d_head)
 
+    # ---- drafted tokens and the int8 KV cache (no counterpart in the reference)
+    # start / lens: the context rows of each sequence (its drafted row i lies at
+    # cache row len + i); parents: [n_seq, rows] or [rows], an earlier row, -1
+    # (the context) or -2 (no node); None: row i follows row i - 1
+    @staticmethod
+    def qk_norm_rope(qkv, start, rows, n_q, n_kv, head_dim, freqs, q_weight=None, k_weight=None, eps=1e-5, q_scale=1.0,
+                     parents=None) -> tuple[Storage, Storage, Storage]:
+        """Per-head RMSNorm of q and k (with a weight) and RoPE at start + depth
+        of the fused qkv rows [n_seq * rows, (n_q + 2 n_kv) * head_dim]."""
+        st = _starts(start)
+        _pa, pp = _parents(parents, st.size, rows)
+        q, k, v = _out(), _out(), _out()
+        call("scry_hip_qk_norm_rope", qkv.h, st.size, rows, st.ctypes.data, pp, n_q, n_kv, head_dim, freqs.h,
+             q_weight.h if q_weight is not None else None, k_weight.h if k_weight is not None else None, eps, q_scale,
+             C.byref(q), C.byref(k), C.byref(v))
+        n = st.size * rows * head_dim
+        return _st(q, n * n_q), _st(k, n * n_kv), _st(v, n * n_kv)
+
+    @staticmethod
+    def kv8_new(max_seq, n_kv, head_dim) -> KvCache8:
+        o = _out()
+        call("scry_hip_kv8_new", max_seq, n_kv, head_dim, C.byref(o))
+        return KvCache8(o.value, max_seq, n_kv, head_dim)
+
+    @staticmethod
+    def kv8_write(caches, k, v, start, rows) -> None:
+        """Quantise k, v [n_seq * rows, n_kv * head_dim] into rows start ..
+        start + rows of the sequences' caches."""
+        st = _starts(start)
+        call("scry_hip_kv8_write", _handles(caches, st.size), st.size, st.ctypes.data, rows, k.h, v.h)
+
+    @staticmethod
+    def kv8_read(caches, start, rows) -> tuple[Storage, Storage]:
+        """Rows start .. start + rows of the caches as f32 k and v [n_seq * rows,
+        n_kv * head_dim]."""
+        st = _starts(start)
+        k, v = _out(), _out()
+        call("scry_hip_kv8_read", _handles(caches, st.size), st.size, st.ctypes.data, rows, C.byref(k), C.byref(v))
+        n = st.size * rows * caches[0].n_kv * caches[0].head_dim
+        return _st(k, n), _st(v, n)
+
+    @staticmethod
+    def kv8_keep(caches, start, paths) -> None:
+        """The accepted paths' rows move up: row start + paths[s][i] to start + i
+        (paths [n_seq, n], each ended by -1 or by n: as verify_tree returns)."""
+        st = _starts(start)
+        p = _ints(paths)
+        if p.ndim != 2 or p.shape[0] != st.size:
+            raise ValueError(f"paths must be [{st.size}, n]")
+        call("scry_hip_kv8_keep", _handles(caches, st.size), st.size, st.ctypes.data, p.ctypes.data, p.shape[1])
+
+    @staticmethod
+    def tree_attention(q, k_caches, v_caches, lens, rows, n_q, n_kv, head_dim, scale, parents=None) -> Storage:
+        """Attention of drafted rows q [n_seq * rows, n_q * head_dim] over f32
+        caches of rows [n_kv * head_dim]: the context and each row's ancestors."""
+        st = _starts(lens)
+        _pa, pp = _parents(parents, st.size, rows)
+        o = _out()
+        call("scry_hip_tree_attention", q.h, _handles(k_caches, st.size), _handles(v_caches, st.size), st.size,
+             st.ctypes.data, rows, pp, n_q, n_kv, head_dim, scale, C.byref(o))
+        return _st(o, q.n)
+
+    @staticmethod
+    def kv8_tree_attention(q, caches, lens, rows, n_q, scale, parents=None) -> Storage:
+        """tree_attention over int8 caches."""
+        st = _starts(lens)
+        _pa, pp = _parents(parents, st.size, rows)
+        o = _out()
+        call("scry_hip_kv8_tree_attention", q.h, _handles(caches, st.size), st.size, st.ctypes.data, rows, pp, n_q, scale,
+             C.byref(o))
+        return _st(o, q.n)
+
+    @staticmethod
+    def verify_draft(p, q, tokens, u, vocab, counts=None) -> tuple[np.ndarray, np.ndarray]:
+        """A drafted chain per sequence against the target's probabilities: p
+        [n_seq, rows + 1, vocab], q [n_seq, rows, vocab], tokens [n_seq, rows], u
+        [n_seq, rows + 1]; returns (accepted [n_seq], next token [n_seq])."""
+        t = _ints(tokens, np.int64)
+        if t.ndim != 2:
+            raise ValueError("tokens must be [n_seq, rows]")
+        n_seq, rows = t.shape
+        r = np.ascontiguousarray(u, np.float64)
+        if r.shape != (n_seq, rows + 1):
+            raise ValueError(f"u must be [{n_seq}, {rows + 1}]")
+        c = None if counts is None else _ints(counts)
+        if c is not None and c.shape != (n_seq,):
+            raise ValueError("one count per sequence")
+        n, token = np.empty(n_seq, np.int64), np.empty(n_seq, np.int64)
+        call("scry_hip_verify_draft", p.h, q.h, t.ctypes.data, None if c is None else c.ctypes.data, r.ctypes.data, n_seq,
+             rows, vocab, n.ctypes.data, token.ctypes.data)
+        return n, token
+
+    @staticmethod
+    def verify_tree(p, tokens, parents, u, vocab) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+        """A drafted tree per sequence: p [n_seq, rows + 1, vocab] (row 0 after
+        the context, row 1 + i after node i), tokens [n_seq, rows], u [n_seq,
+        rows + 1]; returns (paths [n_seq, rows], ended by -1; accepted [n_seq];
+        next token [n_seq])."""
+        t = _ints(tokens, np.int64)
+        if t.ndim != 2:
+            raise ValueError("tokens must be [n_seq, rows]")
+        n_seq, rows = t.shape
+        r = np.ascontiguousarray(u, np.float64)
+        if r.shape != (n_seq, rows + 1):
+            raise ValueError(f"u must be [{n_seq}, {rows + 1}]")
+        _pa, pp = _parents(parents, n_seq, rows)
+        paths = np.empty((n_seq, rows), np.int64)
+        n, token = np.empty(n_seq, np.int64), np.empty(n_seq, np.int64)
+        call("scry_hip_verify_tree", p.h, t.ctypes.data, pp, r.ctypes.data, n_seq, rows, vocab, paths.ctypes.data,
+             n.ctypes.data, token.ctypes.data)
+        return paths, n, token
+
 
 def init(device: int = 0) -> None:
     HipBackend.init_gpu(device)
 
 
-__all__ = ["HipBackend", "Storage", "I8Storage", "init", "_lib"]
+__all__ = ["HipBackend", "Storage", "I8Storage", "KvCache8", "init", "_lib"]

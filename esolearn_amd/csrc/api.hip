@@ -115,12 +115,30 @@ int new_buf(size_t n, scry_buf *out) {
 }
 
 void del_buf(scry_buf b) {
-    if (!b) return;
+    if (!b || --b->refs > 0) return;
     pool_free(b->d);
     pool_free(b->bf);
     pool_free(b->pk);
     delete b;
 }
+
+// A DLPack managed tensor (the public exchange format: data, device, rank,
+// element type, shape, strides, offset; a context and a deleter) that holds a
+// storage.
+struct DlView {
+    struct {
+        void *data;
+        int32_t device_type, device_id, ndim;
+        uint8_t type_code, type_bits;
+        uint16_t type_lanes;
+        int64_t *shape, *strides;
+        uint64_t byte_offset;
+    } t;
+    void *ctx;
+    void (*deleter)(DlView *);
+    scry_buf buf;
+    int64_t shape;
+};
 
 // a failed op leaves no output behind
 int keep_out(int rc, scry_buf *out) {
@@ -340,6 +358,15 @@ int qmatmul(scry_buf a, scry_i8buf bq, float scale, const float *scales32, const
 
 }  // namespace
 
+namespace scry {
+int buf_new(size_t n, scry_buf *out) { return new_buf(n, out); }
+void buf_del(scry_buf b) { del_buf(b); }
+int check_f32(scry_buf b, const char *what) {
+    CHECK_BUF(b, what);
+    return SCRY_OK;
+}
+}  // namespace scry
+
 extern "C" {
 
 // ------------------------------------------------------------------ runtime
@@ -390,6 +417,7 @@ int scry_hip_shutdown(void) {
     Ctx &c = ctx();
     if (!c.init) return SCRY_OK;
     (void)hipStreamSynchronize(c.stream);
+    host_block_free();
     pool_trim();
     dev_free(c.ws);
     (void)hipStreamDestroy(c.stream);
@@ -542,6 +570,47 @@ int scry_hip_clone_storage(scry_buf src, scry_buf *out) {
 int scry_hip_buf_len(scry_buf b, size_t *n) {
     if (!b || !n) return set_error(SCRY_ERR_INVALID, "buf_len: null argument");
     *n = b->n;
+    return SCRY_OK;
+}
+
+int scry_hip_buf_dlpack(scry_buf b, void *wait_stream, int wait, void **managed) {
+    API_LOCK;
+    SCRY_REQUIRE_INIT();
+    if (!managed) return set_error(SCRY_ERR_INVALID, "buf_dlpack: null output");
+    *managed = nullptr;
+    CHECK_BUF(b, "buf_dlpack");
+    DeviceScope dev;
+    if (wait) {  // what the caller's stream does next comes after what the storage's values still wait for
+        hipEvent_t e = nullptr;
+        SCRY_HIP(hipEventCreateWithFlags(&e, hipEventDisableTiming));
+        hipError_t r = hipEventRecord(e, ctx().stream);
+        if (r == hipSuccess) r = hipStreamWaitEvent((hipStream_t)wait_stream, e, 0);
+        (void)hipEventDestroy(e);
+        SCRY_HIP(r);
+    }
+    auto *v = new (std::nothrow) DlView;
+    if (!v) return set_error(SCRY_ERR_OOM, "host allocation failed");
+    bf16_stale(b);  // the caller may write through the view
+    b->refs++;
+    v->buf = b;
+    v->shape = (int64_t)b->n;
+    v->t.data = b->d;
+    v->t.device_type = 10;  // ROCm
+    v->t.device_id = ctx().device;
+    v->t.ndim = 1;
+    v->t.type_code = 2;  // float
+    v->t.type_bits = 32;
+    v->t.type_lanes = 1;
+    v->t.shape = &v->shape;
+    v->t.strides = nullptr;
+    v->t.byte_offset = 0;
+    v->ctx = nullptr;
+    v->deleter = [](DlView *x) {
+        API_LOCK;
+        del_buf(x->buf);
+        delete x;
+    };
+    *managed = v;
     return SCRY_OK;
 }
 

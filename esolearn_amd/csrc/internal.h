@@ -37,6 +37,25 @@ int set_error(int code, const char *fmt, ...);
 int hip_fail(hipError_t e, const char *expr, const char *file, int line);
 int dev_alloc(void **p, size_t bytes);
 void dev_free(void *p);
+// op storage (api.hip): a new one of n values, and its end
+int buf_new(size_t n, scry_buf *out);
+void buf_del(scry_buf b);
+// f32 storage, neither null nor bf16-only
+int check_f32(scry_buf b, const char *what);
+// The library's device is the thread's current one while this lives, so that
+// an op's allocations and launches go there whatever the caller had selected.
+struct DeviceScope {
+    int back = -1;
+    DeviceScope() {
+        int d = -1;
+        if (hipGetDevice(&d) == hipSuccess && d != ctx().device && hipSetDevice(ctx().device) == hipSuccess) back = d;
+    }
+    ~DeviceScope() {
+        if (back >= 0) (void)hipSetDevice(back);
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+};
 // pool.hip: device blocks for op storage and op temporaries, used on the
 // context's stream only; freed blocks are reused in stream order
 int pool_alloc(void **p, size_t bytes);
@@ -435,6 +454,22 @@ bool attn_prefill_planes(int hd);  // head sizes the bf16 plane attention takes
 int launch_attn_prefill(const PrefillAttn &a, int n_seq, const PrefillSeqs &t, int l, const PrefillKVP &kv,
                         hipStream_t s);
 
+// draft.hip -- what the ops on drafted tokens share
+constexpr int DRAFT_MAX_TREE = 64;  // nodes of a tree: an ancestor set is one 64-bit mask
+constexpr int DRAFT_MAX_HD = 256;   // head sizes: multiples of 4 up to here
+struct DraftBatch {                 // passed to kernels by value
+    int n_seq, rows, tree;          // tree: 0 = row i's parent is row i - 1
+    int len[PF_MAX_SEQS];           // context rows of each sequence: row i lies at len + i
+    signed char parent[PF_MAX_SEQS][DRAFT_MAX_TREE];  // tree: -1 the context, -2 no node
+};
+// Checks start and parents (host, [n_seq] and [n_seq][rows] or null) and fills b.
+int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, const int32_t *parents, DraftBatch *b);
+int check_heads(const char *what, int n_q, int n_kv, int head_dim);  // n_q = 0: no query heads
+// pinned host memory that the device reads and writes, `bytes` large, kept until shutdown; its users wait
+// for the stream before they return
+int host_block(size_t bytes, void **p);
+void host_block_free();
+
 // bf16.hip -- bf16 mode: the reference's cast, widening, B-operand rows
 // [n][kp] (kp = bf16_row_pad(k)), the GEMM activation plane, the bf16 GEMV
 int bf16_row_pad(int k);
@@ -472,6 +507,17 @@ struct scry_buf_s {
     // logical (pk_k, pk_n, pk_tb), built on first use
     unsigned short *pk = nullptr;
     int pk_k = 0, pk_n = 0, pk_kp = 0, pk_tb = -1;
+    int refs = 1;  // the handle, and every device view of it
+};
+
+// One layer's int8 KV cache of one sequence (kv8.hip has the layout)
+struct scry_kv8_s {
+    int8_t *k = nullptr, *v = nullptr;
+    float *ks = nullptr, *vs = nullptr;
+    int max_seq = 0, n_kv = 0, hd = 0;
+    int hdp = 0;     // hd rounded up to 16
+    int rows_p = 0;  // max_seq rounded up to 64
+    char *block = nullptr;
 };
 
 struct scry_i8buf_s {

@@ -21,7 +21,7 @@
  *    synchronise, as the reference's to_vec does.  Calls from several host
  *    threads are serialised internally.
  *  - Only float32 storage and int8 weight storage exist, as in the
- *    reference's `quantize` feature (W8A32).
+ *    reference's `quantize` feature (W8A32), and int8 KV caches (scry_kv8).
  */
 #ifndef SCRY_HIP_H
 #define SCRY_HIP_H
@@ -47,6 +47,7 @@ typedef struct scry_buf_s *scry_buf;     /* f32 device storage (Storage)       *
 typedef struct scry_i8buf_s *scry_i8buf; /* int8 weight storage (I8Storage)    */
 typedef struct scry_llama_s *scry_llama; /* LlamaModel with int8 projections   */
 typedef struct scry_kv_cache_s *scry_kv_cache; /* LlamaKvCache (device)        */
+typedef struct scry_kv8_s *scry_kv8;     /* int8 KV cache of one layer and sequence */
 
 /* SamplingConfig (generate.rs:24-45): temperature (< 1e-8 means greedy),
  * top_k (0 or >= vocab: off), top_p (outside (0, 1): off), max_tokens. */
@@ -91,6 +92,16 @@ int scry_hip_to_vec(scry_buf b, float *host, size_t n);
 /* DeviceBackend::clone_storage (mod.rs:44) */
 int scry_hip_clone_storage(scry_buf src, scry_buf *out);
 int scry_hip_buf_len(scry_buf b, size_t *n);
+/* A storage's f32 values where they lie on the device, for other device code
+ * of the process: *managed is a DLPack DLManagedTensor, to be ended by its
+ * deleter; until then the values stay, also after scry_hip_free.  (No
+ * counterpart in the reference.)  The library works on a stream of its own:
+ * with wait != 0 what wait_stream (a hipStream_t, null: the default one) is
+ * given next comes after the ops called so far; with wait = 0, and before
+ * values written through the view are used or the view ends, the caller
+ * orders the two sides (scry_hip_synchronize, hipStreamSynchronize).  Take a
+ * new view to write to a storage that a bf16-mode matmul has read. */
+int scry_hip_buf_dlpack(scry_buf b, void *wait_stream, int wait, void **managed);
 int scry_hip_free(scry_buf b);
 
 /* DeviceBackend::i8_from_vec (mod.rs:17-18, `quantize` feature) */
@@ -243,6 +254,80 @@ int scry_hip_split_qkv_reshape_heads(scry_buf qkv, int seq, int n_heads, int d_h
 int scry_hip_reshape_for_heads(scry_buf x, int batch, int seq, int n_heads, int d_head, scry_buf *out);
 /* MathBackend::reshape_from_heads (mod.rs:484-510): the inverse */
 int scry_hip_reshape_from_heads(scry_buf x, int batch, int seq, int n_heads, int d_head, scry_buf *out);
+
+/* ------------------------------------------- drafted tokens, int8 KV cache
+ * No counterpart in the reference, which decodes one token of one sequence at
+ * a time over an f32 cache (llama.rs:371-468, generate.rs:51-89).
+ *
+ * A batch is n_seq sequences (1 to 16) of `rows` drafted tokens each; all
+ * arrays of ints are host arrays.  start / len [n_seq]: the context rows of
+ * each sequence; its drafted row i lies at cache row len + i.  parents
+ * [n_seq][rows], or null: row i follows row i - 1 (one new token, a drafted
+ * chain, a chunk of a prompt; any number of rows).  With parents the rows are
+ * a tree (at most 64): an earlier row, -1: the context, -2: no node (what pads
+ * a smaller tree; its row of an attention is zero, and no node's parent).
+ * head_dim: a multiple of 4, at most 256. */
+
+/* Per-head RMSNorm of q and k, and RoPE, in one pass over the fused qkv rows
+ * [n_seq * rows, (n_q + 2 n_kv) * head_dim]: n = h / sqrt(mean(h^2) + eps) *
+ * weight (q_weight, k_weight [head_dim]; null: h as it is), then the rotation
+ * of rope_with_freqs_preloaded (adjacent pairs, freqs [head_dim / 2], f64
+ * angles) at position start + depth, a row's depth being the number of its
+ * ancestors.  q is also multiplied by q_scale; v is copied.  Outputs [n_seq *
+ * rows, n_q * head_dim] and twice [n_seq * rows, n_kv * head_dim]. */
+int scry_hip_qk_norm_rope(scry_buf qkv, int n_seq, int rows, const int32_t *start, const int32_t *parents, int n_q,
+                          int n_kv, int head_dim, scry_buf freqs, scry_buf q_weight, scry_buf k_weight, float eps,
+                          float q_scale, scry_buf *q, scry_buf *k, scry_buf *v);
+
+/* An int8 KV cache of max_seq rows of one layer and one sequence: a quarter of
+ * the f32 cache's bytes, plus one f32 scale per row and head. */
+int scry_hip_kv8_new(int max_seq, int n_kv, int head_dim, scry_kv8 *out);
+int scry_hip_kv8_free(scry_kv8 c);
+/* Quantise k, v [n_seq * rows, n_kv * head_dim] into rows start .. start + rows
+ * of the sequences' caches (distinct, of one shape).  Per row and head: s =
+ * f32(max|x| / 127), q = x / s to the nearest integer, halves away from zero.
+ * A row of zeros has s = 0; one with an infinity or NaN has s = NaN. */
+int scry_hip_kv8_write(const scry_kv8 *caches, int n_seq, const int32_t *start, int rows, scry_buf k, scry_buf v);
+/* Rows start .. start + rows read back: f32(q) * s, [n_seq * rows, n_kv *
+ * head_dim].  Rows never written are zero. */
+int scry_hip_kv8_read(const scry_kv8 *caches, int n_seq, const int32_t *start, int rows, scry_buf *k, scry_buf *v);
+/* The accepted path's rows move up: row start + paths[s][i] to start + i, for
+ * every i below n_path (at most 64) or the first -1.  A path is ascending
+ * nodes below 64; it may be empty. */
+int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, const int32_t *paths, int n_path);
+
+/* Attention of the drafted rows: q [n_seq * rows, n_q * head_dim]; row i of a
+ * sequence attends to its cache rows [0, len) and to len + j of its ancestors j
+ * and of itself: softmax(scale * q.k) v, n_q / n_kv query heads per KV head.
+ * Keys outside that set may hold anything.  The f32 form reads caches of rows
+ * [n_kv * head_dim] (what scatter_rows fills), at least len + rows of them. */
+int scry_hip_tree_attention(scry_buf q, const scry_buf *k_caches, const scry_buf *v_caches, int n_seq, const int32_t *len,
+                            int rows, const int32_t *parents, int n_q, int n_kv, int head_dim, float scale, scry_buf *out);
+int scry_hip_kv8_tree_attention(scry_buf q, const scry_kv8 *caches, int n_seq, const int32_t *len, int rows,
+                                const int32_t *parents, int n_q, float scale, scry_buf *out);
+
+/* Verification of drafted tokens against the target's probabilities (rows of
+ * softmax), with given random numbers u in [0, 1).  A draw from weights w with
+ * u is the lowest j with w_0 + .. + w_j > u * sum(w), in f64; weights not
+ * positive and finite count as zero.  1 <= rows <= 64.  Results are host
+ * values: the calls wait for them.
+ *
+ * verify_draft: a chain.  p [n_seq][rows + 1][vocab], q [n_seq][rows][vocab]
+ * (what each token was drawn from), tokens [n_seq][rows], u [n_seq][rows + 1];
+ * counts [n_seq] (null: rows) tokens of a sequence are drafted.  accepted =
+ * the first i with not (u_i q_i(x_i) < p_i(x_i)), or count; token is drawn with
+ * the sequence's last u from max(p_i - q_i, 0) there (from p_i where that is
+ * zero throughout), or from p_count.  Where p has no mass, every token has the
+ * same weight. */
+int scry_hip_verify_draft(scry_buf p, scry_buf q, const int64_t *tokens, const int32_t *counts, const double *u, int n_seq,
+                          int rows, int vocab, int64_t *accepted, int64_t *token);
+/* verify_tree: p [n_seq][rows + 1][vocab], row 0 after the context, row 1 + i
+ * after node i; a token is drawn from row r with u [n_seq][rows + 1] (r); from
+ * row 0 the walk follows the child (the lowest) whose token is the drawn one.
+ * paths [n_seq][rows]: the accepted nodes, then -1; accepted [n_seq]; token
+ * [n_seq]: the token drawn from the last row. */
+int scry_hip_verify_tree(scry_buf p, const int64_t *tokens, const int32_t *parents, const double *u, int n_seq, int rows,
+                         int vocab, int64_t *paths, int64_t *accepted, int64_t *token);
 
 /* ------------------------------------------------------ Llama (llama.rs) */
 typedef struct {
