@@ -12,8 +12,8 @@
 // bytes of a row being an operand of the products q.k; V [head][row / 64][hdp]
 // [64], the 64 rows of a block side by side per dimension, in the order in
 // which a wave's scores of those rows lie in its lanes (kv8_perm), so that a
-// lane's 16 bytes are an operand of the products p.v; hdp = hd rounded up to
-// 16, the padding zero.  Scales [head][row].
+// lane's 16 bytes make an operand of the products p.v; V's bytes are q + 128.
+// hdp = hd rounded up to 16.  Scales [head][row].
 #include <cmath>
 #include <new>
 
@@ -97,10 +97,10 @@ __global__ __launch_bounds__(256) void k_kv8_write(Kv8Rows a, const float *__res
     if (is_v) {
         if (act) {
             int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, g, r, 4 * gl) + kv8_perm(r & 63);
-            d[0] = q.x;
-            d[64] = q.y;
-            d[128] = q.z;
-            d[192] = q.w;
+            d[0] = q.x ^ 0x80;
+            d[64] = q.y ^ 0x80;
+            d[128] = q.z ^ 0x80;
+            d[192] = q.w ^ 0x80;
         }
     } else if (act) {
         *(char4 *)(a.c.k[s] + kv8_k_at(rows_p, hdp, g, r) + 4 * gl) = q;
@@ -121,7 +121,8 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Rows a, float *__restrict__
     char4 q;
     if (is_v) {
         const int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, g, r, 4 * gl) + kv8_perm(r & 63);
-        q = make_char4(d[0], d[64], d[128], d[192]);
+        q = make_char4((signed char)(d[0] ^ 0x80), (signed char)(d[64] ^ 0x80), (signed char)(d[128] ^ 0x80),
+                       (signed char)(d[192] ^ 0x80));
     } else {
         q = *(const char4 *)(a.c.k[s] + kv8_k_at(rows_p, hdp, g, r) + 4 * gl);
     }
