@@ -115,6 +115,17 @@ __device__ __forceinline__ float col_sum(float v) {
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Four dimensions of column c's output: o times 1 / l, or zero where there is no node.
+__device__ __forceinline__ void store_out(const TreeArgs &a, int s, int g, int c, int d, float4 o, float inv) {
+    const int node = c / a.nrep, h = g * a.nrep + c % a.nrep;
+    float4 r = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (a.d.tree && a.d.parent[s][node] == -2) r = make_float4(0.f, 0.f, 0.f, 0.f);
+    *(float4 *)(a.out + (((size_t)s * a.d.rows + node) * a.n_q + h) * a.hd + d) = r;
+}
+__device__ __forceinline__ size_t part_of(const TreeArgs &a, const Unit &u, int c) {
+    return (((size_t)u.s * a.n_kv + u.g) * a.cols + c) * a.n_split + u.split;
+}
+
 // The four waves' (c, sum, out) of each column joined in wave order, from
 // s_o [wave][column][ld], s_c and s_l [wave][column]: the output, or one split's
 // partial.  Factors are 2^(c - max c); a wave without keys has c = -inf.
@@ -142,61 +153,73 @@ __device__ __forceinline__ void join_waves(const TreeArgs &a, const Unit &u, con
             o.z += v.z * f;
             o.w += v.w * f;
         }
-        const int node = c / a.nrep, h = u.g * a.nrep + c % a.nrep;
         if (a.n_split == 1) {
-            float4 r = make_float4(o.x / L, o.y / L, o.z / L, o.w / L);
-            if (a.d.tree && a.d.parent[u.s][node] == -2) r = make_float4(0.f, 0.f, 0.f, 0.f);
-            *(float4 *)(a.out + (((size_t)u.s * a.d.rows + node) * a.n_q + h) * hd + d) = r;
+            store_out(a, u.s, u.g, c, d, o, 1.f / L);
         } else {
-            const size_t at = (((size_t)u.s * a.n_kv + u.g) * a.cols + c) * a.n_split + u.split;
+            const size_t at = part_of(a, u, c);
             *(float4 *)(a.part_o + at * hd + d) = o;
             if (d == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(C, L);
         }
     }
 }
 
-// The splits of a column joined in split order: a wave per column, a lane per
-// four dimensions (and per split, for the factors).
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col) {
-    const size_t col = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (col >= n_col) return;
-    const int c = (int)(col % a.cols), g = (int)(col / a.cols % a.n_kv), s = (int)(col / a.cols / a.n_kv);
-    const int node = c / a.nrep, h = g * a.nrep + c % a.nrep, hd = a.hd;
-    const float *ml = a.part_ml + col * a.n_split * 2;
-    float cc = -INFINITY, l = 0.f;
-    if (lane < a.n_split) {
-        cc = ml[2 * lane];
-        l = ml[2 * lane + 1];
-    }
-    float C = cc;
+// The splits of a column joined in a fixed order.  A workgroup takes `per`
+// columns: a wave finds a column's factors, a lane per split; then 256 / per
+// threads sum its splits, lanes of four dimensions times groups of splits, and
+// the groups are joined through LDS.
+constexpr int MAX_SPLIT = 64;
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col, int per, int lanes) {
+    __shared__ float s_f[16 * MAX_SPLIT], s_l[16];
+    __shared__ float4 s_p[256];
+    const int tid = threadIdx.x, lane = tid & 63, hd = a.hd, ns = a.n_split;
+    const size_t col0 = (size_t)blockIdx.x * per;
+    for (int i = tid >> 6; i < per && col0 + i < n_col; i += 4) {
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < ns) ml = *(const float2 *)(a.part_ml + ((col0 + i) * ns + lane) * 2);
+        float C = ml.x;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) C = fmaxf(C, __shfl_xor(C, off));
-    const float f = exp2_fast(cc - (C == -INFINITY ? 0.f : C));
-    const float L = wave_sum(l * f);
-    const bool act = 4 * lane < hd;
-    const float *o = a.part_o + col * a.n_split * hd + 4 * lane;
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int p = 0; p < a.n_split; p++) {
-        const float fp = __shfl(f, p);
-        const float4 v = act ? *(const float4 *)(o + (size_t)p * hd) : r;
-        r.x += v.x * fp;
-        r.y += v.y * fp;
-        r.z += v.z * fp;
-        r.w += v.w * fp;
+        for (int off = 32; off > 0; off >>= 1) C = fmaxf(C, __shfl_xor(C, off));
+        const float f = exp2_fast(ml.x - (C == -INFINITY ? 0.f : C));
+        const float L = wave_sum(ml.y * f);
+        if (lane < ns) s_f[i * MAX_SPLIT + lane] = f;
+        if (lane == 0) s_l[i] = L;
     }
-    if (!act) return;
-    r = make_float4(r.x / L, r.y / L, r.z / L, r.w / L);
-    if (a.d.tree && a.d.parent[s][node] == -2) r = make_float4(0.f, 0.f, 0.f, 0.f);
-    *(float4 *)(a.out + (((size_t)s * a.d.rows + node) * a.n_q + h) * hd + 4 * lane) = r;
+    __syncthreads();
+    const int n_grp = 256 / (per * lanes), x = tid % lanes, grp = tid / lanes % n_grp, i = tid / (lanes * n_grp);
+    const size_t col = col0 + i;
+    const bool act = col < n_col && 4 * x < hd;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (act) {
+        const float *o = a.part_o + col * ns * hd + 4 * x;
+#pragma unroll 8
+        for (int p = grp; p < ns; p += n_grp) {
+            const float f = s_f[i * MAX_SPLIT + p];
+            const float4 v = *(const float4 *)(o + (size_t)p * hd);
+            r.x += v.x * f;
+            r.y += v.y * f;
+            r.z += v.z * f;
+            r.w += v.w * f;
+        }
+    }
+    s_p[tid] = r;
+    __syncthreads();
+    if (grp || !act) return;
+    for (int k = 1; k < n_grp; k++) {
+        const float4 v = s_p[tid + k * lanes];
+        r.x += v.x;
+        r.y += v.y;
+        r.z += v.z;
+        r.w += v.w;
+    }
+    const int c = (int)(col % a.cols), g = (int)(col / a.cols % a.n_kv), s = (int)(col / a.cols / a.n_kv);
+    store_out(a, s, g, c, 4 * x, r, 1.f / s_l[i]);
 }
 
 // The steps of SK keys that a workgroup takes of the keys that its columns see.
-template <int SK, int COLS>
-__device__ __forceinline__ void step_range(const TreeArgs &a, const Unit &u, int *lo, int *hi) {
+template <int SK>
+__device__ __forceinline__ void step_range(const TreeArgs &a, const Unit &u, int cols, int *lo, int *hi) {
     int rows = a.d.rows;
-    if (!a.d.tree) rows = min(rows, (min(a.cols, (u.qg + 1) * COLS) - 1) / a.nrep + 1);
+    if (!a.d.tree) rows = min(rows, (min(a.cols, (u.qg + 1) * cols) - 1) / a.nrep + 1);
     const long long steps = ((long long)a.d.len[u.s] + rows + SK - 1) / SK;
     *lo = (int)(steps * u.split / a.n_split);
     *hi = (int)(steps * (u.split + 1) / a.n_split);
@@ -211,81 +234,172 @@ __device__ __forceinline__ void step_range(const TreeArgs &a, const Unit &u, int
 // the largest w is 2^14, and f16's smallest steps lie 2^-38 below.  Scales
 // below 2^-80 count as 2^-80 there, which keeps 2^-c in f32's range.
 // KS: steps of 64 dimensions (hdp <= 64 KS).
-template <int KS, int QT>
+
+// Column c's query as digits: lane (cl, j) holds dimensions 64 k + 16 j ..;
+// returns what a score's integer is multiplied by (but the key's scale).
+template <int KS>
+__device__ __forceinline__ float query_digits(const TreeArgs &a, const Unit &u, int c, int j, i32x4 (&qd)[3][KS]) {
+    const int cc = min(c, a.cols - 1), node = cc / a.nrep, rep = cc % a.nrep, hd = a.hd;
+    const float *q = a.q + (((size_t)u.s * a.d.rows + node) * a.n_q + u.g * a.nrep + rep) * hd;
+    float4 x[KS][4];
+    float m = 0.f;
+    bool fin = true;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = 64 * k + 16 * j + 4 * e;
+            x[k][e] = d < hd ? *(const float4 *)(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 v = x[k][e];
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            fin &= isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
+        }
+    // a query with an infinity or NaN has no finite softmax over any key
+    m = col_max(fin ? fmaxf(m, 0x1p-96f) : INFINITY);
+    const float up = m < INFINITY ? 8290000.f / m : 0.f;  // 126.5 * 2^16: the top digit stays below 128
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float v[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
+            unsigned w[3] = {0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int X = up > 0.f ? (int)rintf(v[i] * up) : 0;
+                const int d0 = (int)(signed char)X, X1 = (X - d0) >> 8, d1 = (int)(signed char)X1, d2 = (X1 - d1) >> 8;
+                w[0] |= (unsigned)(d0 & 255) << (8 * i);
+                w[1] |= (unsigned)(d1 & 255) << (8 * i);
+                w[2] |= (unsigned)(d2 & 255) << (8 * i);
+            }
+#pragma unroll
+            for (int g = 0; g < 3; g++) qd[g][k][e] = (int)w[g];
+        }
+    return m < INFINITY ? m / 8290000.f * a.scale2 : __builtin_nanf("");
+}
+
+// The integer scores of 16 keys, digits joined: (h 256 + b), each exact.
+template <int KS>
+__device__ __forceinline__ f32x4 digit_scores(const i32x4 (&kk)[KS], const i32x4 (&qd)[3][KS]) {
+    i32x4 h = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < KS; k++) h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[k], qd[2][k], h, 0, 0, 0);
+    h = h << 8;  // (|h| <= 2^22: hd products of two digits)
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+        h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[k], qd[1][k], h, 0, 0, 0);
+        b = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[k], qd[0][k], b, 0, 0, 0);
+    }
+    f32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = fmaf((float)h[i], 256.f, (float)b[i]);
+    return r;
+}
+
+// A column's running state: largest score, exponent of the largest scale - 14,
+// sum of the weights.
+struct RunI8 {
+    float m = -INFINITY, ve = -94.f, l = 0.f;
+};
+
+// One step's 64 scores of a column (16 a lane; key 16 x + 4 j + i at [x][i])
+// and the rows' scales into the operands of w.v.  Where the reference moves,
+// l is rescaled and o's factor is returned (1: o stays).  FULL: every key is seen.
+template <bool FULL>
+__device__ __forceinline__ float softmax_step(RunI8 &r, f32x4 (&sc)[4], const f32x4 (&vs)[4], const Column &co, int t, int len,
+                                              f16x8 (&wh)[2], f16x8 (&wl)[2]) {
+    float vm = 0.f, mx = -INFINITY;
+    unsigned seen = 0;
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (FULL) {
+                vm = fmaxf(vm, vs[x][i]);
+            } else {
+                const bool in = sees(co, t + 16 * x + i, len);
+                seen |= (unsigned)in << (4 * x + i);
+                sc[x][i] = in ? sc[x][i] : -INFINITY;
+                vm = fmaxf(vm, in ? vs[x][i] : 0.f);
+            }
+            mx = fmaxf(mx, sc[x][i]);
+        }
+    vm = col_max(vm);
+    mx = fmaxf(r.m, col_max(mx));
+    // 2^e >= the largest scale, e >= -80
+    const float e = fmaxf(r.ve, (float)((int)((__float_as_uint(fmaxf(vm, 0x1p-80f)) + 0x7fffffu) >> 23) - 127 - 14));
+    const float ref = mx == -INFINITY ? 0.f : mx + e;
+    float al = 1.f;
+    if (__any(mx != r.m || e != r.ve)) {
+        al = r.m == -INFINITY ? 0.f : exp2_fast(r.m + r.ve - ref);
+        r.l *= al;
+        r.m = mx;
+        r.ve = e;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float p = exp2_fast(sc[x][i] - ref);
+            sum += p;
+            w[i] = p * vs[x][i];
+            if (!FULL && !(seen >> (4 * x + i) & 1)) w[i] = 0.f;  // the scale may be NaN
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 1]));
+            const f16x2 lo = __builtin_bit_cast(
+                f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf(-(float)h[0], 1.f, w[i]), fmaf(-(float)h[1], 1.f, w[i + 1])));
+            wh[x / 2][4 * (x % 2) + i] = h[0];
+            wh[x / 2][4 * (x % 2) + i + 1] = h[1];
+            wl[x / 2][4 * (x % 2) + i] = lo[0];
+            wl[x / 2][4 * (x % 2) + i + 1] = lo[1];
+        }
+    }
+    r.l += sum;
+    return al;
+}
+
+// Eight of a dimension's V bytes (two words of four rows) as f16: byte v + 128
+// behind 0x64 is 1024 + v + 128.
+__device__ __forceinline__ f16x8 v_operand(int w0, int w1) {
+    i32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        r[i] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, (unsigned)(i < 2 ? w0 : w1),
+                                                                                        i % 2 ? 0x04030402u : 0x04010400u)) -
+                                           f16x2{(_Float16)1152.f, (_Float16)1152.f});
+    return __builtin_bit_cast(f16x8, r);
+}
+
+// Few columns (one tile a workgroup): bound by reading the cache.  Keys go
+// from memory to the operands, every wave with steps of its own.
+template <int KS>
 __global__ __launch_bounds__(64 * WAVES, KS <= 3 ? 2 : 1) void k_tree_i8(TreeArgs a, Kv8Batch cb) {
-    constexpr int DT = 4 * KS, COLS = 16 * QT;
+    constexpr int DT = 4 * KS, COLS = 16;
     extern __shared__ __align__(16) float sm[];
     Unit u;
     if (!unit_of(a, u)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int cl = lane & 15, j = lane >> 4;
     const int hd = a.hd, hdp = cb.hdp, len = a.d.len[u.s];
-
-    // the columns' queries as digits: lane (cl, j) holds dimensions 64 x + 16 j ..
-    const unsigned long long anc = a.d.tree ? ancestor_mask(a.d, u.s) : 0;
-    Column co[QT];
-    i32x4 qd[QT][3][KS];
-    float qs[QT];
+    const int c = u.qg * COLS + cl;
+    const Column co = column_of(a, u.s, c, a.d.tree ? ancestor_mask(a.d, u.s) : 0);
+    i32x4 qd[3][KS];
+    const float qs = query_digits<KS>(a, u, c, j, qd);
+    RunI8 r;
+    f32x4 o[DT];
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const int c = u.qg * COLS + 16 * t + cl;
-        co[t] = column_of(a, u.s, c, anc);
-        const int node = min(c, a.cols - 1) / a.nrep, rep = min(c, a.cols - 1) % a.nrep;
-        const float *q = a.q + (((size_t)u.s * a.d.rows + node) * a.n_q + u.g * a.nrep + rep) * hd;
-        float4 x[KS][4];
-        float m = 0.f;
-        bool fin = true;
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int d = 64 * k + 16 * j + 4 * e;
-                x[k][e] = d < hd ? *(const float4 *)(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float4 v = x[k][e];
-                m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-                fin &= isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
-            }
-        // a query with an infinity or NaN has no finite softmax over any key
-        m = col_max(fin ? fmaxf(m, 0x1p-96f) : INFINITY);
-        const float up = m < INFINITY ? 8290000.f / m : 0.f;  // 126.5 * 2^16: the top digit stays below 128
-        qs[t] = m < INFINITY ? m / 8290000.f * a.scale2 : __builtin_nanf("");
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float v[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
-                unsigned w[3] = {0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int X = up > 0.f ? (int)rintf(v[i] * up) : 0;
-                    const int d0 = (int)(signed char)X, X1 = (X - d0) >> 8, d1 = (int)(signed char)X1, d2 = (X1 - d1) >> 8;
-                    w[0] |= (unsigned)(d0 & 255) << (8 * i);
-                    w[1] |= (unsigned)(d1 & 255) << (8 * i);
-                    w[2] |= (unsigned)(d2 & 255) << (8 * i);
-                }
-#pragma unroll
-                for (int g = 0; g < 3; g++) qd[t][g][k][e] = (int)w[g];
-            }
-    }
-
-    float m[QT], ve[QT], l[QT];  // largest score, exponent of the largest scale - 14, sum
-    f32x4 o[QT][DT];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        m[t] = -INFINITY;
-        ve[t] = -94.f;
-        l[t] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < DT; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int rows_p = cb.rows_p[u.s];
     const int8_t *kb = cb.k[u.s] + (size_t)u.g * rows_p * hdp, *vb = cb.v[u.s] + (size_t)u.g * rows_p * hdp;
     const float *ksb = cb.ks[u.s] + (size_t)u.g * rows_p, *vsb = cb.vs[u.s] + (size_t)u.g * rows_p;
     int lo, hi;
-    step_range<64, COLS>(a, u, &lo, &hi);
+    step_range<64>(a, u, COLS, &lo, &hi);
 
     i32x4 kk[4][KS];
-    float4 ks[4];
+    f32x4 ks[4];
     auto load_k = [&](int st) {
         const int8_t *kt = kb + (size_t)st * 64 * hdp;
 #pragma unroll
@@ -293,145 +407,160 @@ __global__ __launch_bounds__(64 * WAVES, KS <= 3 ? 2 : 1) void k_tree_i8(TreeArg
 #pragma unroll
             for (int k = 0; k < KS; k++)
                 kk[x][k] = 64 * k + 16 * j < hdp ? *(const i32x4 *)(kt + (16 * x + cl) * hdp + 64 * k + 16 * j) : i32x4{0, 0, 0, 0};
-            ks[x] = *(const float4 *)(ksb + st * 64 + 16 * x + 4 * j);
+            ks[x] = *(const f32x4 *)(ksb + st * 64 + 16 * x + 4 * j);
         }
     };
     if (lo + wave < hi) load_k(lo + wave);
     for (int st = lo + wave; st < hi; st += WAVES) {
         const int t0 = st * 64;
         const int8_t *vt = vb + (size_t)t0 * hdp;
-        float4 vs[4];
+        f32x4 vs[4], sc[4];
 #pragma unroll
-        for (int x = 0; x < 4; x++) vs[x] = *(const float4 *)(vsb + t0 + 16 * x + 4 * j);
-        i32x4 vv[DT];
-
-        const bool full = t0 + 64 <= len;  // every column sees every key
-        float vmax = 0.f;
-        if (full) {
+        for (int x = 0; x < 4; x++) vs[x] = *(const f32x4 *)(vsb + t0 + 16 * x + 4 * j);
 #pragma unroll
-            for (int x = 0; x < 4; x++) vmax = fmaxf(vmax, fmaxf(fmaxf(vs[x].x, vs[x].y), fmaxf(vs[x].z, vs[x].w)));
-            vmax = col_max(vmax);
-        }
-        f16x8 wh[QT][2], wl[QT][2];
+        for (int x = 0; x < 4; x++) sc[x] = digit_scores<KS>(kk[x], qd) * (ks[x] * qs);
+        i32x4 vv[DT];  // K is used up: its registers take V
 #pragma unroll
-        for (int t = 0; t < QT; t++) {
-            float sc[4][4];
-            float mx = -INFINITY;
+        for (int d = 0; d < DT; d++)
+            vv[d] = 16 * d < hdp ? *(const i32x4 *)(vt + (16 * d + cl) * 64 + 16 * j) : i32x4{0, 0, 0, 0};
+        f16x8 wh[2], wl[2];
+        const float al = t0 + 64 <= len ? softmax_step<true>(r, sc, vs, co, t0 + 4 * j, len, wh, wl)
+                                        : softmax_step<false>(r, sc, vs, co, t0 + 4 * j, len, wh, wl);
+        if (__any(al != 1.f)) {
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                i32x4 h = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-#pragma unroll
-                for (int k = 0; k < KS; k++) h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[x][k], qd[t][2][k], h, 0, 0, 0);
-                // (|h| <= 2^22: hd products of two digits)
-                h = h << 8;
-#pragma unroll
-                for (int k = 0; k < KS; k++) h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[x][k], qd[t][1][k], h, 0, 0, 0);
-#pragma unroll
-                for (int k = 0; k < KS; k++) b = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[x][k], qd[t][0][k], b, 0, 0, 0);
-                const float kx[4] = {ks[x].x, ks[x].y, ks[x].z, ks[x].w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) sc[x][i] = fmaf((float)h[i], 256.f, (float)b[i]) * (qs[t] * kx[i]);
-            }
-            if (t == QT - 1) {  // K is used up: its registers take V
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-                    vv[d] = 16 * d < hdp ? *(const i32x4 *)(vt + (16 * d + cl) * 64 + 16 * j) : i32x4{0, 0, 0, 0};
-            }
-            float vm = vmax;
-            unsigned seen = 0xffffu;
-            if (!full) {
-                seen = 0;
-                vm = 0.f;
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const float vx[4] = {vs[x].x, vs[x].y, vs[x].z, vs[x].w};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const bool in = sees(co[t], t0 + 16 * x + 4 * j + i, len);
-                        seen |= (unsigned)in << (4 * x + i);
-                        sc[x][i] = in ? sc[x][i] : -INFINITY;
-                        vm = fmaxf(vm, in ? vx[i] : 0.f);
-                    }
-                }
-                vm = col_max(vm);
-            }
-#pragma unroll
-            for (int x = 0; x < 4; x++) mx = fmaxf(mx, fmaxf(fmaxf(sc[x][0], sc[x][1]), fmaxf(sc[x][2], sc[x][3])));
-            mx = fmaxf(m[t], col_max(mx));
-            // 2^e >= the largest scale, e >= -80
-            const float e = fmaxf(ve[t], (float)((int)((__float_as_uint(fmaxf(vm, 0x1p-80f)) + 0x7fffffu) >> 23) - 127 - 14));
-            const float ref = mx == -INFINITY ? 0.f : mx + e;
-            if (__any(mx != m[t] || e != ve[t])) {
-                const float al = m[t] == -INFINITY ? 0.f : exp2_fast(m[t] + ve[t] - ref);
-                l[t] *= al;
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[t][d] *= al;
-                m[t] = mx;
-                ve[t] = e;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const float vx[4] = {vs[x].x, vs[x].y, vs[x].z, vs[x].w};
-                float w[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float p = exp2_fast(sc[x][i] - ref);
-                    sum += p;
-                    w[i] = p * vx[i];
-                    if (!full && !(seen >> (4 * x + i) & 1)) w[i] = 0.f;  // the scale may be NaN
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 1]));
-                    const f16x2 r = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[i] - (float)h[0], w[i + 1] - (float)h[1]));
-                    wh[t][x / 2][4 * (x % 2) + i] = h[0];
-                    wh[t][x / 2][4 * (x % 2) + i + 1] = h[1];
-                    wl[t][x / 2][4 * (x % 2) + i] = r[0];
-                    wl[t][x / 2][4 * (x % 2) + i + 1] = r[1];
-                }
-            }
-            l[t] += sum;
+            for (int d = 0; d < DT; d++) o[d] *= al;
         }
         load_k(min(st + WAVES, hi - 1));  // under the products below
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
+        for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                // byte b = v + 128 behind 0x64 is f16 1024 + b
-                i32x4 hv;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const unsigned by = (unsigned)vv[d][2 * x + i / 2];
-                    const f16x2 r = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, by, i % 2 ? 0x04030402u : 0x04010400u)) -
-                                    f16x2{(_Float16)1152.f, (_Float16)1152.f};
-                    hv[i] = __builtin_bit_cast(int, r);
-                }
-                const f16x8 va = __builtin_bit_cast(f16x8, hv);
-#pragma unroll
-                for (int t = 0; t < QT; t++) {
-                    o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wh[t][x], o[t][d], 0, 0, 0);
-                    o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl[t][x], o[t][d], 0, 0, 0);
-                }
+                const f16x8 va = v_operand(vv[d][2 * x], vv[d][2 * x + 1]);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wh[x], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl[x], o[d], 0, 0, 0);
             }
-        }
     }
 
-    const int ld = hd + 4;
+    const int ld = hd + 4, col = wave * COLS + cl;
     float *s_o = sm, *s_c = sm + WAVES * COLS * ld, *s_l = s_c + WAVES * COLS;
+    const float sum = col_sum(r.l);
+    if (j == 0) {
+        s_c[col] = r.m == -INFINITY ? r.m : r.m + r.ve;
+        s_l[col] = sum;
+    }
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const int col = wave * COLS + 16 * t + cl;
-        const float sum = col_sum(l[t]);
-        if (j == 0) {
-            s_c[col] = m[t] == -INFINITY ? m[t] : m[t] + ve[t];
-            s_l[col] = sum;
+    for (int d = 0; d < DT; d++)
+        if (16 * d + 4 * j < hd) *(f32x4 *)(s_o + col * ld + 16 * d + 4 * j) = o[d];
+    join_waves<COLS>(a, u, s_o, s_c, s_l, ld);
+}
+
+// Many columns: bound by the arithmetic of the softmax and the conversions, so
+// W waves with a tile each share the keys through LDS: each stages a part of
+// a step, V as f16 (converted once for the W tiles), in the order in which the
+// lanes take their operands, and holds the next step's part in registers.
+template <int KS, int W>
+__global__ __launch_bounds__(64 * W, KS == 1 ? 4 : KS == 2 ? 3 : 2) void k_tree_i8_wide(TreeArgs a, Kv8Batch cb) {
+    constexpr int DT = 4 * KS, XB = (4 + W - 1) / W, DB = (DT + W - 1) / W;
+    __shared__ i32x4 s_k[4][KS][64];
+    __shared__ f16x8 s_v[DT][2][64];
+    __shared__ f32x4 s_sc[2][16];  // scales of K and V
+    Unit u;
+    if (!unit_of(a, u)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cl = lane & 15, j = lane >> 4;
+    const int hd = a.hd, hdp = cb.hdp, len = a.d.len[u.s];
+    const int c0 = (u.qg * W + wave) * 16, c = c0 + cl;
+    const Column co = column_of(a, u.s, c, a.d.tree ? ancestor_mask(a.d, u.s) : 0);
+    i32x4 qd[3][KS];
+    const float qs = query_digits<KS>(a, u, c, j, qd);
+    // keys that any column of this wave sees
+    const int end = c0 >= a.cols ? 0 : a.d.tree ? len + a.d.rows : len + min(c0 + 15, a.cols - 1) / a.nrep + 1;
+    RunI8 r;
+    f32x4 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int rows_p = cb.rows_p[u.s];
+    const int8_t *kb = cb.k[u.s] + (size_t)u.g * rows_p * hdp, *vb = cb.v[u.s] + (size_t)u.g * rows_p * hdp;
+    const float *scb = (tid < 64 ? cb.ks[u.s] : cb.vs[u.s]) + (size_t)u.g * rows_p + lane;
+    int lo, hi;
+    step_range<64>(a, u, 16 * W, &lo, &hi);
+
+    i32x4 kr[XB][KS], vr[DB];
+    float sr = 0.f;
+    auto fetch = [&](int st) {
+        const int8_t *kt = kb + (size_t)st * 64 * hdp, *vt = vb + (size_t)st * 64 * hdp;
+#pragma unroll
+        for (int b = 0; b < XB; b++)
+            if (W * b + wave < 4)
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+                    kr[b][k] = 64 * k + 16 * j < hdp ? *(const i32x4 *)(kt + (16 * (W * b + wave) + cl) * hdp + 64 * k + 16 * j)
+                                                     : i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+            vr[b] = 16 * (W * b + wave) < hdp ? *(const i32x4 *)(vt + (16 * (W * b + wave) + cl) * 64 + 16 * j) : i32x4{0, 0, 0, 0};
+        if (tid < 128) sr = scb[(size_t)st * 64];
+    };
+    if (lo < hi) fetch(lo);
+    for (int st = lo; st < hi; st++) {
+        const int t0 = st * 64;
+        __syncthreads();  // the step before has been read
+#pragma unroll
+        for (int b = 0; b < XB; b++)
+            if (W * b + wave < 4)
+#pragma unroll
+                for (int k = 0; k < KS; k++) s_k[W * b + wave][k][lane] = kr[b][k];
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+            if (W * b + wave < DT) {
+                s_v[W * b + wave][0][lane] = v_operand(vr[b][0], vr[b][1]);
+                s_v[W * b + wave][1][lane] = v_operand(vr[b][2], vr[b][3]);
+            }
+        if (tid < 128) ((float *)s_sc)[tid] = sr;
+        __syncthreads();
+        fetch(min(st + 1, hi - 1));
+        if (t0 >= end) continue;  // (uniform in the wave)
+        f32x4 sc[4], vs[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            i32x4 kk[KS];
+#pragma unroll
+            for (int k = 0; k < KS; k++) kk[k] = s_k[x][k][lane];
+            sc[x] = digit_scores<KS>(kk, qd) * (s_sc[0][4 * x + j] * qs);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; x++) vs[x] = s_sc[1][4 * x + j];
+        f16x8 wh[2], wl[2];
+        const float al = t0 + 64 <= len ? softmax_step<true>(r, sc, vs, co, t0 + 4 * j, len, wh, wl)
+                                        : softmax_step<false>(r, sc, vs, co, t0 + 4 * j, len, wh, wl);
+        if (__any(al != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= al;
         }
 #pragma unroll
         for (int d = 0; d < DT; d++)
-            if (16 * d + 4 * j < hd) *(f32x4 *)(s_o + col * ld + 16 * d + 4 * j) = o[t][d];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const f16x8 va = s_v[d][x][lane];
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wh[x], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl[x], o[d], 0, 0, 0);
+            }
     }
-    join_waves<COLS>(a, u, s_o, s_c, s_l, ld);
+
+    const float sum = col_sum(r.l);
+    if (c >= a.cols) return;
+    const size_t at = part_of(a, u, c);
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        const int dd = 16 * d + 4 * j;
+        if (dd >= hd) break;
+        const float4 v = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+        if (a.n_split == 1)
+            store_out(a, u.s, u.g, c, dd, v, 1.f / sum);
+        else
+            *(float4 *)(a.part_o + at * hd + dd) = v;
+    }
+    if (a.n_split > 1 && j == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(r.m == -INFINITY ? r.m : r.m + r.ve, sum);
 }
 
 // ------------------------------------------------------------- f32 cache
@@ -442,9 +571,9 @@ __global__ __launch_bounds__(64 * WAVES, KS <= 3 ? 2 : 1) void k_tree_i8(TreeArg
 // rows 4 j + i as float4 of dimensions 64 e + 4 cl .., so every load is 16
 // bytes wide and a row's lanes are neighbours.
 // ET: blocks of 64 dimensions.
-template <int ET, int QT>
+template <int ET>
 __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeArgs a, F32Batch fb) {
-    constexpr int CT = 4 * ET, COLS = 16 * QT;
+    constexpr int CT = 4 * ET, COLS = 16, QT = 1;
     extern __shared__ __align__(16) float sm[];
     Unit u;
     if (!unit_of(a, u)) return;
@@ -474,15 +603,21 @@ __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeAr
     }
     const float *kb = fb.k[u.s] + (size_t)u.g * hd, *vb = fb.v[u.s] + (size_t)u.g * hd;
     int lo, hi;
-    step_range<16, COLS>(a, u, &lo, &hi);
+    step_range<16>(a, u, COLS, &lo, &hi);
 
+    f32x4 kk[CT];
+    auto load_k = [&](int st) {
+        const float *kt = kb + (size_t)st * 16 * ldk + (size_t)cl * ldk + 4 * j;
+        const bool in = cl < end - st * 16;
+#pragma unroll
+        for (int x = 0; x < CT; x++) kk[x] = in && 16 * x + 4 * j < hd ? *(const f32x4 *)(kt + 16 * x) : zero;
+    };
+    if (lo + wave < hi) load_k(lo + wave);
     for (int st = lo + wave; st < hi; st += WAVES) {
         const int t0 = st * 16;
-        const float *kt = kb + (size_t)t0 * ldk, *vt = vb + (size_t)t0 * ldk;
+        const float *vt = vb + (size_t)t0 * ldk;
         const int left = end - t0;  // rows that there are, from t0 on
-        f32x4 kk[CT], vv[4][ET];
-#pragma unroll
-        for (int x = 0; x < CT; x++) kk[x] = cl < left && 16 * x + 4 * j < hd ? *(const f32x4 *)(kt + (size_t)cl * ldk + 16 * x + 4 * j) : zero;
+        f32x4 vv[4][ET];
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -490,23 +625,7 @@ __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeAr
                 vv[i][e] = 4 * j + i < left && 64 * e + 4 * cl < hd ? *(const f32x4 *)(vt + (size_t)(4 * j + i) * ldk + 64 * e + 4 * cl) : zero;
 
         const bool full = t0 + 16 <= len;
-        // In drafted rows a value that is not finite may be seen by one column
-        // and not by another: 0 * inf must not reach the latter.  Such values
-        // leave the products here and are added one by one below.
         bool odd = false;
-        if (!full) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int e = 0; e < ET; e++)
-#pragma unroll
-                    for (int f = 0; f < 4; f++)
-                        if (!isfinite(vv[i][e][f])) {
-                            odd = true;
-                            vv[i][e][f] = 0.f;
-                        }
-            odd = __any(odd);
-        }
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             f32x4 s0 = zero, s1 = zero;
@@ -518,6 +637,23 @@ __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeAr
                     s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[x][e], q[t][x][e], s0, 0, 0, 0);
                     s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[x][e + 1], q[t][x][e + 1], s1, 0, 0, 0);
                 }
+            }
+            if (t == QT - 1) load_k(min(st + WAVES, hi - 1));  // K is used up: under the products p.v
+            // In drafted rows a value that is not finite may be seen by one column
+            // and not by another: 0 * inf must not reach the latter.  Such values
+            // leave the products here and are added one by one below.
+            if (!full && t == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < ET; e++)
+#pragma unroll
+                        for (int f = 0; f < 4; f++)
+                            if (!isfinite(vv[i][e][f])) {
+                                odd = true;
+                                vv[i][e][f] = 0.f;
+                            }
+                odd = __any(odd);
             }
             float sc[4];
             float mx = -INFINITY;
@@ -596,26 +732,24 @@ __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeAr
     join_waves<COLS>(a, u, s_o, s_c, s_l, ld);
 }
 
-constexpr int MAX_SPLIT = 64;  // k_tree_merge has a lane per split
-
-// Key splits: enough workgroups to fill the chip, each wave with a few steps.
-int pick_splits(const TreeArgs &a, int step_keys) {
+// Key splits: about `want` workgroups, each with at least `least` steps.
+int pick_splits(const TreeArgs &a, int step_keys, int want, int least) {
     int len = 0;
     for (int s = 0; s < a.d.n_seq; s++) len = len > a.d.len[s] ? len : a.d.len[s];
     const long long steps = ((long long)len + a.d.rows + step_keys - 1) / step_keys;
     const long long units = (long long)a.d.n_seq * a.n_kv * a.n_qg;
-    long long n = (768 + units - 1) / units;
-    const long long most = steps / (2 * WAVES);
+    long long n = (want + units - 1) / units;
+    const long long most = steps / least;
     if (n > most) n = most;
     if (n > MAX_SPLIT) n = MAX_SPLIT;
     return n < 1 ? 1 : (int)n;
 }
 
+// waves: of a workgroup; cols: its columns
 template <class K, class B>
-int launch_tree(K kernel, TreeArgs a, const B &b, int qt, int step_keys, hipStream_t s) {
-    const int cols = 16 * qt;
+int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t lds, int step_keys, int want, int least, hipStream_t s) {
     a.n_qg = (a.cols + cols - 1) / cols;
-    a.n_split = pick_splits(a, step_keys);
+    a.n_split = pick_splits(a, step_keys, want, least);
     const size_t n_col = (size_t)a.d.n_seq * a.n_kv * a.cols;
     void *ws = nullptr;
     SCRY_TRY(split_workspace(n_col * (a.hd + 2) * sizeof(float), &a.n_split, &ws));
@@ -624,15 +758,44 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int qt, int step_keys, hipStre
     a.n_pair = a.d.n_seq * a.n_kv * a.n_split;
     const size_t grid = (size_t)((a.n_pair + 7) / 8) * 8 * a.n_qg;
     if (grid > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "attention: %zu workgroups", grid);
-    const size_t lds = (size_t)WAVES * cols * (a.hd + 4 + 2) * sizeof(float);
-    SCRY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WAVES), lds, s, a, b);
+    if (lds > 65536)
+        SCRY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), lds, s, a, b);
     SCRY_HIP(hipGetLastError());
     if (a.n_split > 1) {
-        hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((n_col + 3) / 4)), dim3(256), 0, s, a, n_col);
+        int lanes = 1;
+        while (4 * lanes < a.hd) lanes *= 2;
+        // threads of a column: its lanes, times up to as many groups as it has splits
+        int per = 256 / lanes;
+        while (per > 1 && 256 / (per * lanes) * 2 <= a.n_split) per /= 2;
+        if (per > 16) per = 16;
+        hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((n_col + per - 1) / per)), dim3(256), 0, s, a, n_col, per, lanes);
         SCRY_HIP(hipGetLastError());
     }
     return SCRY_OK;
+}
+
+#ifndef WANT1
+#define WANT1 768
+#define LEAST1 8
+#define WANTW 768
+#define LEASTW 4
+#define WANTF 768
+#define LEASTF 8
+#endif
+template <int KS>
+int launch_i8(const TreeArgs &a, const Kv8Batch &b, hipStream_t s) {
+    const int tiles = (a.cols + 15) / 16, groups = (tiles + 3) / 4, w = (tiles + groups - 1) / groups;
+    const size_t lds = (size_t)WAVES * 16 * (a.hd + 4 + 2) * sizeof(float);
+    if (w == 1) return launch_tree(k_tree_i8<KS>, a, b, WAVES, 16, lds, 64, WANT1, LEAST1, s);
+    if (w == 2) return launch_tree(k_tree_i8_wide<KS, 2>, a, b, 2, 32, 0, 64, 2 * WANTW, LEASTW, s);
+    if (w == 3) return launch_tree(k_tree_i8_wide<KS, 3>, a, b, 3, 48, 0, 64, 4 * WANTW / 3, LEASTW, s);
+    return launch_tree(k_tree_i8_wide<KS, 4>, a, b, 4, 64, 0, 64, WANTW, LEASTW, s);
+}
+template <int ET>
+int launch_f32(const TreeArgs &a, const F32Batch &b, hipStream_t s) {
+    const size_t lds = (size_t)WAVES * 16 * (a.hd + 4 + 2) * sizeof(float);
+    return launch_tree(k_tree_f32<ET>, a, b, WAVES, 16, lds, 16, WANTF, LEASTF, s);
 }
 
 int tree_run(const char *what, scry_buf q, const TreeArgs &t, bool i8, const F32Batch &f, const Kv8Batch &c, scry_buf *out) {
@@ -649,18 +812,14 @@ int tree_run(const char *what, scry_buf q, const TreeArgs &t, bool i8, const F32
     a.out = o->d;
     hipStream_t s = ctx().stream;
     const int blocks = (a.hd + 63) / 64;
-    const bool two = a.cols > 16;  // two tiles a wave where there are two
-    int rc;
-    if (i8)
-        rc = blocks == 1   ? two ? launch_tree(k_tree_i8<1, 2>, a, c, 2, 64, s) : launch_tree(k_tree_i8<1, 1>, a, c, 1, 64, s)
-             : blocks == 2 ? two ? launch_tree(k_tree_i8<2, 2>, a, c, 2, 64, s) : launch_tree(k_tree_i8<2, 1>, a, c, 1, 64, s)
-             : blocks == 3 ? launch_tree(k_tree_i8<3, 1>, a, c, 1, 64, s)
-                           : launch_tree(k_tree_i8<4, 1>, a, c, 1, 64, s);
-    else
-        rc = blocks == 1   ? two ? launch_tree(k_tree_f32<1, 2>, a, f, 2, 16, s) : launch_tree(k_tree_f32<1, 1>, a, f, 1, 16, s)
-             : blocks == 2 ? two ? launch_tree(k_tree_f32<2, 2>, a, f, 2, 16, s) : launch_tree(k_tree_f32<2, 1>, a, f, 1, 16, s)
-             : blocks == 3 ? launch_tree(k_tree_f32<3, 1>, a, f, 1, 16, s)
-                           : launch_tree(k_tree_f32<4, 1>, a, f, 1, 16, s);
+    const int rc = i8 ? blocks == 1   ? launch_i8<1>(a, c, s)
+                        : blocks == 2 ? launch_i8<2>(a, c, s)
+                        : blocks == 3 ? launch_i8<3>(a, c, s)
+                                      : launch_i8<4>(a, c, s)
+                   : blocks == 1 ? launch_f32<1>(a, f, s)
+                   : blocks == 2 ? launch_f32<2>(a, f, s)
+                   : blocks == 3 ? launch_f32<3>(a, f, s)
+                                 : launch_f32<4>(a, f, s);
     if (rc) {
         buf_del(o);
         return rc;
