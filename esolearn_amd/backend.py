@@ -8,6 +8,7 @@ lives on the GPU; ``to_vec`` copies back to numpy.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 
@@ -136,17 +137,25 @@ def _ints(a, dtype=np.int32) -> np.ndarray:
     x = np.ascontiguousarray(a)
     if x.dtype != dtype:
         y = x.astype(dtype)
-        if not np.array_equal(x, y):
+        if (x != y).any():
             raise ValueError(f"expected values that {np.dtype(dtype).name} holds")
         x = y
     return x
 
 
-def _starts(start) -> np.ndarray:
-    a = _ints(start)
-    if a.ndim != 1:
-        raise ValueError("one context length per sequence")
-    return a
+def _at(a: np.ndarray) -> int:
+    """Where an array's values lie (ndarray.ctypes takes 1 us)."""
+    return a.__array_interface__["data"][0]
+
+
+def _starts(start) -> array:
+    """One context length per sequence, as C ints."""
+    try:
+        if getattr(start, "ndim", 1) == 1:
+            return array("i", start)
+    except (TypeError, OverflowError):
+        pass
+    raise ValueError("one context length per sequence, as whole numbers below 2^31")
 
 
 def _parents(parents, n_seq: int, rows: int):
@@ -158,13 +167,13 @@ def _parents(parents, n_seq: int, rows: int):
         a = np.ascontiguousarray(np.broadcast_to(a, (n_seq, rows)))
     if a.shape != (n_seq, rows):
         raise ValueError(f"parents must be [{n_seq}, {rows}] or [{rows}]")
-    return a, a.ctypes.data
+    return a, _at(a)
 
 
-def _handles(items, n_seq: int):
+def _handles(items, n_seq: int) -> array:
     if len(items) != n_seq:
         raise ValueError("one cache per sequence")
-    return (C.c_void_p * n_seq)(*[i.h for i in items])
+    return array("Q", [i.h or 0 for i in items])
 
 
 def _st(h: C.c_void_p, n: int) -> Storage:
@@ -540,12 +549,13 @@ class HipBackend:
         """Per-head RMSNorm of q and k (with a weight) and RoPE at start + depth
         of the fused qkv rows [n_seq * rows, (n_q + 2 n_kv) * head_dim]."""
         st = _starts(start)
-        _pa, pp = _parents(parents, st.size, rows)
+        n_seq = len(st)
+        _pa, pp = _parents(parents, n_seq, rows)
         q, k, v = _out(), _out(), _out()
-        call("scry_hip_qk_norm_rope", qkv.h, st.size, rows, st.ctypes.data, pp, n_q, n_kv, head_dim, freqs.h,
+        call("scry_hip_qk_norm_rope", qkv.h, n_seq, rows, st.buffer_info()[0], pp, n_q, n_kv, head_dim, freqs.h,
              q_weight.h if q_weight is not None else None, k_weight.h if k_weight is not None else None, eps, q_scale,
              C.byref(q), C.byref(k), C.byref(v))
-        n = st.size * rows * head_dim
+        n = n_seq * rows * head_dim
         return _st(q, n * n_q), _st(k, n * n_kv), _st(v, n * n_kv)
 
     @staticmethod
@@ -559,16 +569,20 @@ class HipBackend:
         """Quantise k, v [n_seq * rows, n_kv * head_dim] into rows start ..
         start + rows of the sequences' caches."""
         st = _starts(start)
-        call("scry_hip_kv8_write", _handles(caches, st.size), st.size, st.ctypes.data, rows, k.h, v.h)
+        n_seq = len(st)
+        h = _handles(caches, n_seq)
+        call("scry_hip_kv8_write", h.buffer_info()[0], n_seq, st.buffer_info()[0], rows, k.h, v.h)
 
     @staticmethod
     def kv8_read(caches, start, rows) -> tuple[Storage, Storage]:
         """Rows start .. start + rows of the caches as f32 k and v [n_seq * rows,
         n_kv * head_dim]."""
         st = _starts(start)
+        n_seq = len(st)
+        h = _handles(caches, n_seq)
         k, v = _out(), _out()
-        call("scry_hip_kv8_read", _handles(caches, st.size), st.size, st.ctypes.data, rows, C.byref(k), C.byref(v))
-        n = st.size * rows * caches[0].n_kv * caches[0].head_dim
+        call("scry_hip_kv8_read", h.buffer_info()[0], n_seq, st.buffer_info()[0], rows, C.byref(k), C.byref(v))
+        n = n_seq * rows * caches[0].n_kv * caches[0].head_dim
         return _st(k, n), _st(v, n)
 
     @staticmethod
@@ -576,29 +590,35 @@ class HipBackend:
         """The accepted paths' rows move up: row start + paths[s][i] to start + i
         (paths [n_seq, n], each ended by -1 or by n: as verify_tree returns)."""
         st = _starts(start)
+        n_seq = len(st)
         p = _ints(paths)
-        if p.ndim != 2 or p.shape[0] != st.size:
-            raise ValueError(f"paths must be [{st.size}, n]")
-        call("scry_hip_kv8_keep", _handles(caches, st.size), st.size, st.ctypes.data, p.ctypes.data, p.shape[1])
+        if p.ndim != 2 or p.shape[0] != n_seq:
+            raise ValueError(f"paths must be [{n_seq}, n]")
+        h = _handles(caches, n_seq)
+        call("scry_hip_kv8_keep", h.buffer_info()[0], n_seq, st.buffer_info()[0], _at(p), p.shape[1])
 
     @staticmethod
     def tree_attention(q, k_caches, v_caches, lens, rows, n_q, n_kv, head_dim, scale, parents=None) -> Storage:
         """Attention of drafted rows q [n_seq * rows, n_q * head_dim] over f32
         caches of rows [n_kv * head_dim]: the context and each row's ancestors."""
         st = _starts(lens)
-        _pa, pp = _parents(parents, st.size, rows)
+        n_seq = len(st)
+        _pa, pp = _parents(parents, n_seq, rows)
+        hk, hv = _handles(k_caches, n_seq), _handles(v_caches, n_seq)
         o = _out()
-        call("scry_hip_tree_attention", q.h, _handles(k_caches, st.size), _handles(v_caches, st.size), st.size,
-             st.ctypes.data, rows, pp, n_q, n_kv, head_dim, scale, C.byref(o))
+        call("scry_hip_tree_attention", q.h, hk.buffer_info()[0], hv.buffer_info()[0], n_seq, st.buffer_info()[0], rows, pp,
+             n_q, n_kv, head_dim, scale, C.byref(o))
         return _st(o, q.n)
 
     @staticmethod
     def kv8_tree_attention(q, caches, lens, rows, n_q, scale, parents=None) -> Storage:
         """tree_attention over int8 caches."""
         st = _starts(lens)
-        _pa, pp = _parents(parents, st.size, rows)
+        n_seq = len(st)
+        _pa, pp = _parents(parents, n_seq, rows)
+        h = _handles(caches, n_seq)
         o = _out()
-        call("scry_hip_kv8_tree_attention", q.h, _handles(caches, st.size), st.size, st.ctypes.data, rows, pp, n_q, scale,
+        call("scry_hip_kv8_tree_attention", q.h, h.buffer_info()[0], n_seq, st.buffer_info()[0], rows, pp, n_q, scale,
              C.byref(o))
         return _st(o, q.n)
 
@@ -618,8 +638,8 @@ class HipBackend:
         if c is not None and c.shape != (n_seq,):
             raise ValueError("one count per sequence")
         n, token = np.empty(n_seq, np.int64), np.empty(n_seq, np.int64)
-        call("scry_hip_verify_draft", p.h, q.h, t.ctypes.data, None if c is None else c.ctypes.data, r.ctypes.data, n_seq,
-             rows, vocab, n.ctypes.data, token.ctypes.data)
+        call("scry_hip_verify_draft", p.h, q.h, _at(t), None if c is None else _at(c), _at(r), n_seq,
+             rows, vocab, _at(n), _at(token))
         return n, token
 
     @staticmethod
@@ -638,8 +658,8 @@ class HipBackend:
         _pa, pp = _parents(parents, n_seq, rows)
         paths = np.empty((n_seq, rows), np.int64)
         n, token = np.empty(n_seq, np.int64), np.empty(n_seq, np.int64)
-        call("scry_hip_verify_tree", p.h, t.ctypes.data, pp, r.ctypes.data, n_seq, rows, vocab, paths.ctypes.data,
-             n.ctypes.data, token.ctypes.data)
+        call("scry_hip_verify_tree", p.h, _at(t), pp, _at(r), n_seq, rows, vocab, _at(paths),
+             _at(n), _at(token))
         return paths, n, token
 
 

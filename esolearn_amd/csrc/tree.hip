@@ -42,7 +42,10 @@ struct TreeArgs {
     float *out;
     float *part_o, *part_ml;  // n_split > 1: [column][split][hd], [column][split][2] (c, sum)
     int n_q, n_kv, hd, nrep, cols;  // cols = rows * nrep
-    int n_split, n_qg, n_pair;      // key splits, groups of QT tiles, (sequence, KV head, split)s
+    // Key splits of each sequence, alike in size across them; a split's unit is
+    // (sequence, KV head, split), numbered from pair0[s] on.  n_split: the most.
+    int n_split, n_qg;  // n_qg: groups of the workgroup's columns
+    int splits[PF_MAX_SEQS], pair0[PF_MAX_SEQS + 1];
     float scale2;                   // scale * log2(e)
 };
 
@@ -62,11 +65,12 @@ struct Unit {  // a workgroup's part of the work
 __device__ __forceinline__ bool unit_of(const TreeArgs &a, Unit &u) {
     const int i = blockIdx.x, pair = (i & 7) + 8 * ((i >> 3) / a.n_qg);
     u.qg = (i >> 3) % a.n_qg;
-    if (pair >= a.n_pair) return false;  // padding of the last eight
-    u.split = pair % a.n_split;
-    const int sg = pair / a.n_split;
-    u.g = sg % a.n_kv;
-    u.s = sg / a.n_kv;
+    if (pair >= a.pair0[a.d.n_seq]) return false;  // padding of the last eight
+    u.s = 0;
+    while (pair >= a.pair0[u.s + 1]) u.s++;
+    const int at = pair - a.pair0[u.s];
+    u.split = at % a.splits[u.s];
+    u.g = at / a.splits[u.s];
     return true;
 }
 
@@ -104,14 +108,25 @@ __device__ __forceinline__ bool sees(const Column &c, int t, int len) {
     return t < c.lim || ((unsigned)j < 64u && (c.mask >> j & 1));
 }
 
-// Largest value over the four lanes of a column; their sum.
+// Largest value over the four lanes of a column; their sum.  The swaps give
+// every lane its own value and that of the lane 16 (32) away, without LDS.
+__device__ __forceinline__ float2 swap16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float2 swap32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float col_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    float2 p = swap16(v);
+    p = swap32(fmaxf(p.x, p.y));
+    return fmaxf(p.x, p.y);
 }
 __device__ __forceinline__ float col_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    float2 p = swap16(v);
+    p = swap32(p.x + p.y);
+    return p.x + p.y;
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -171,17 +186,18 @@ constexpr int MAX_SPLIT = 64;
 __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col, int per, int lanes) {
     __shared__ float s_f[16 * MAX_SPLIT], s_l[16];
     __shared__ float4 s_p[256];
-    const int tid = threadIdx.x, lane = tid & 63, hd = a.hd, ns = a.n_split;
+    const int tid = threadIdx.x, lane = tid & 63, hd = a.hd;
     const size_t col0 = (size_t)blockIdx.x * per;
+    const auto seq_of = [&](size_t col) { return (int)(col / a.cols / a.n_kv); };
     for (int i = tid >> 6; i < per && col0 + i < n_col; i += 4) {
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < ns) ml = *(const float2 *)(a.part_ml + ((col0 + i) * ns + lane) * 2);
+        if (lane < a.splits[seq_of(col0 + i)]) ml = *(const float2 *)(a.part_ml + ((col0 + i) * a.n_split + lane) * 2);
         float C = ml.x;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) C = fmaxf(C, __shfl_xor(C, off));
         const float f = exp2_fast(ml.x - (C == -INFINITY ? 0.f : C));
         const float L = wave_sum(ml.y * f);
-        if (lane < ns) s_f[i * MAX_SPLIT + lane] = f;
+        s_f[i * MAX_SPLIT + lane] = f;
         if (lane == 0) s_l[i] = L;
     }
     __syncthreads();
@@ -190,7 +206,8 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col, in
     const bool act = col < n_col && 4 * x < hd;
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
     if (act) {
-        const float *o = a.part_o + col * ns * hd + 4 * x;
+        const int ns = a.splits[seq_of(col)];
+        const float *o = a.part_o + col * a.n_split * hd + 4 * x;
 #pragma unroll 8
         for (int p = grp; p < ns; p += n_grp) {
             const float f = s_f[i * MAX_SPLIT + p];
@@ -215,14 +232,56 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col, in
     store_out(a, s, g, c, 4 * x, r, 1.f / s_l[i]);
 }
 
+// Many columns: a thread takes four dimensions of one, its splits eight at a
+// time (loads before their first use: a round trip to memory each time).
+__global__ __launch_bounds__(256) void k_tree_merge_flat(TreeArgs a, size_t n) {
+    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= n) return;
+    const int n4 = a.hd / 4, x = (int)(t % n4);
+    const size_t col = t / n4;
+    const int c = (int)(col % a.cols), g = (int)(col / a.cols % a.n_kv), s = (int)(col / a.cols / a.n_kv), ns = a.splits[s];
+    const float2 *ml = (const float2 *)(a.part_ml + col * a.n_split * 2);
+    const float *o = a.part_o + col * a.n_split * a.hd + 4 * x;
+    float C = -INFINITY, L = 0.f;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < ns; p0 += 8) {
+        float2 m[8];
+        float4 v[8];
+#pragma unroll
+        for (int p = 0; p < 8; p++) {
+            const int q = min(p0 + p, ns - 1);
+            m[p] = ml[q];
+            v[p] = *(const float4 *)(o + (size_t)q * a.hd);
+        }
+        float top = C;
+#pragma unroll
+        for (int p = 0; p < 8; p++) top = fmaxf(top, m[p].x);
+        const float ref = top == -INFINITY ? 0.f : top, f0 = exp2_fast(C - ref);
+        C = top;
+        L *= f0;
+        r = make_float4(r.x * f0, r.y * f0, r.z * f0, r.w * f0);
+#pragma unroll
+        for (int p = 0; p < 8; p++) {
+            if (p0 + p >= ns) break;
+            const float f = exp2_fast(m[p].x - ref);
+            L += m[p].y * f;
+            r.x += v[p].x * f;
+            r.y += v[p].y * f;
+            r.z += v[p].z * f;
+            r.w += v[p].w * f;
+        }
+    }
+    store_out(a, s, g, c, 4 * x, r, 1.f / L);
+}
+
 // The steps of SK keys that a workgroup takes of the keys that its columns see.
 template <int SK>
 __device__ __forceinline__ void step_range(const TreeArgs &a, const Unit &u, int cols, int *lo, int *hi) {
     int rows = a.d.rows;
     if (!a.d.tree) rows = min(rows, (min(a.cols, (u.qg + 1) * cols) - 1) / a.nrep + 1);
     const long long steps = ((long long)a.d.len[u.s] + rows + SK - 1) / SK;
-    *lo = (int)(steps * u.split / a.n_split);
-    *hi = (int)(steps * (u.split + 1) / a.n_split);
+    *lo = (int)(steps * u.split / a.splits[u.s]);
+    *hi = (int)(steps * (u.split + 1) / a.splits[u.s]);
 }
 
 // ------------------------------------------------------------ int8 cache
@@ -230,9 +289,10 @@ __device__ __forceinline__ void step_range(const TreeArgs &a, const Unit &u, int
 // its row's largest value in three balanced int8 digits, so the products and
 // their sums over hd are exact integers.
 // p.v: V's bytes become f16 (exact), and w = p * (the row's scale) is split
-// into two f16 terms, 22 bits.  c = max s + log2(the largest scale seen) - 14:
-// the largest w is 2^14, and f16's smallest steps lie 2^-38 below.  Scales
-// below 2^-80 count as 2^-80 there, which keeps 2^-c in f32's range.
+// into two f16 terms, 22 bits.  c starts as max s + log2(the largest scale) - 8
+// and moves where a w passes 2^15: f16's smallest steps lie 2^-32 below the
+// largest w or further.  Scales below 2^-80 count as 2^-80 there, which keeps
+// 2^-c in f32's range.
 // KS: steps of 64 dimensions (hdp <= 64 KS).
 
 // Column c's query as digits: lane (cl, j) holds dimensions 64 k + 16 j ..;
@@ -262,102 +322,139 @@ __device__ __forceinline__ float query_digits(const TreeArgs &a, const Unit &u, 
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const float v[4] = {x[k][e].x, x[k][e].y, x[k][e].z, x[k][e].w};
-            unsigned w[3] = {0, 0, 0};
+            int X[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int X = up > 0.f ? (int)rintf(v[i] * up) : 0;
-                const int d0 = (int)(signed char)X, X1 = (X - d0) >> 8, d1 = (int)(signed char)X1, d2 = (X1 - d1) >> 8;
-                w[0] |= (unsigned)(d0 & 255) << (8 * i);
-                w[1] |= (unsigned)(d1 & 255) << (8 * i);
-                w[2] |= (unsigned)(d2 & 255) << (8 * i);
+            for (int i = 0; i < 4; i++) X[i] = __float2int_rn(v[i] * up);
+#pragma unroll
+            for (int g = 0; g < 3; g++) {  // a digit is the low byte; with it taken off, (X + 128) >> 8 is left
+                const unsigned w01 = __builtin_amdgcn_perm((unsigned)X[1], (unsigned)X[0], 0x0c0c0400u);
+                const unsigned w23 = __builtin_amdgcn_perm((unsigned)X[3], (unsigned)X[2], 0x0c0c0400u);
+                qd[g][k][e] = (int)__builtin_amdgcn_perm(w23, w01, 0x05040100u);
+#pragma unroll
+                for (int i = 0; i < 4; i++) X[i] = (X[i] + 128) >> 8;
             }
-#pragma unroll
-            for (int g = 0; g < 3; g++) qd[g][k][e] = (int)w[g];
         }
     return m < INFINITY ? m / 8290000.f * a.scale2 : __builtin_nanf("");
 }
 
-// The integer scores of 16 keys, digits joined: (h 256 + b), each exact.
-template <int KS>
-__device__ __forceinline__ f32x4 digit_scores(const i32x4 (&kk)[KS], const i32x4 (&qd)[3][KS]) {
-    i32x4 h = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+// The integer scores of N blocks of 16 keys, digits joined: h 256 + b, the sums
+// h and b exact.  b starts at the bits of 1.5 * 2^23, so that b + 1.5 * 2^23 is
+// an f32 as it stands (|b| < 2^22: hd products of two digits), and h at -192,
+// which its two bytes take back.  The blocks' products are interleaved: a
+// chain of one block's would wait for itself.
+template <int KS, int N>
+__device__ __forceinline__ void digit_scores(const i32x4 (&kk)[N][KS], const i32x4 (&qd)[3][KS], f32x4 *sc) {
+    i32x4 h[N], b[N];
 #pragma unroll
-    for (int k = 0; k < KS; k++) h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[k], qd[2][k], h, 0, 0, 0);
-    h = h << 8;  // (|h| <= 2^22: hd products of two digits)
-#pragma unroll
-    for (int k = 0; k < KS; k++) {
-        h = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[k], qd[1][k], h, 0, 0, 0);
-        b = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[k], qd[0][k], b, 0, 0, 0);
+    for (int x = 0; x < N; x++) {
+        h[x] = i32x4{-192, -192, -192, -192};
+        b[x] = i32x4{0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000};
     }
-    f32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = fmaf((float)h[i], 256.f, (float)b[i]);
-    return r;
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int x = 0; x < N; x++) {
+            h[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[x][k], qd[2][k], h[x], 0, 0, 0);
+            b[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[x][k], qd[0][k], b[x], 0, 0, 0);
+        }
+#pragma unroll
+    for (int x = 0; x < N; x++) h[x] = h[x] << 8;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int x = 0; x < N; x++) h[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[x][k], qd[1][k], h[x], 0, 0, 0);
+#pragma unroll
+    for (int x = 0; x < N; x++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) sc[x][i] = fmaf((float)h[x][i], 256.f, __int_as_float(b[x][i]));
 }
 
-// A column's running state: largest score, exponent of the largest scale - 14,
-// sum of the weights.
+// A column's running state: the reference c, the largest score and the
+// exponent of the largest scale - 8 when it last moved, the sum of the weights.
 struct RunI8 {
-    float m = -INFINITY, ve = -94.f, l = 0.f;
+    float c = -INFINITY, m = -INFINITY, ve = -88.f, l = 0.f;
 };
 
-// One step's 64 scores of a column (16 a lane; key 16 x + 4 j + i at [x][i])
-// and the rows' scales into the operands of w.v.  Where the reference moves,
-// l is rescaled and o's factor is returned (1: o stays).  FULL: every key is seen.
-template <bool FULL>
-__device__ __forceinline__ float softmax_step(RunI8 &r, f32x4 (&sc)[4], const f32x4 (&vs)[4], const Column &co, int t, int len,
-                                              f16x8 (&wh)[2], f16x8 (&wl)[2]) {
-    float vm = 0.f, mx = -INFINITY;
+// Weights as two f16 terms, in the order of the operands of w.v.
+__device__ __forceinline__ void split_weights(const float (&w)[4], int x, f16x8 (&wh)[2], f16x8 (&wl)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 1]));
+        const f16x2 lo = __builtin_bit_cast(
+            f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf(-(float)h[0], 1.f, w[i]), fmaf(-(float)h[1], 1.f, w[i + 1])));
+        wh[x / 2][4 * (x % 2) + i] = h[0];
+        wh[x / 2][4 * (x % 2) + i + 1] = h[1];
+        wl[x / 2][4 * (x % 2) + i] = lo[0];
+        wl[x / 2][4 * (x % 2) + i + 1] = lo[1];
+    }
+}
+
+// One step's 64 scores of a column (16 a lane; key 16 x + 4 j + i at [x][i];
+// sc is multiplied by kq for the score) and the rows' scales into the operands
+// of w.v.  Where the reference moves, l is rescaled and o's factor is returned
+// (1: o stays).  The reference need not be the largest score: it is kept while
+// the weights fit f16 and the sum f32, so most steps neither look for a
+// maximum nor rescale (64-node trees of eight 4000-row contexts: VARIANT).
+template <class KQ, class VS>
+__device__ __forceinline__ float softmax_step(RunI8 &r, const f32x4 (&sc)[4], KQ &&kq, VS &&vs, bool full, const Column &co, int t,
+                                              int len, f16x8 (&wh)[2], f16x8 (&wl)[2]) {
+    if (full) {
+        float sum = 0.f, top = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const f32x4 k = kq(x), v = vs(x);
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = exp2_fast(fmaf(sc[x][i], k[i], -r.c));
+                sum += p;
+                w[i] = p * v[i];
+            }
+            top = fmaxf(fmaxf(top, fmaxf(w[0], w[1])), fmaxf(w[2], w[3]));
+            split_weights(w, x, wh, wl);
+        }
+        // (a NaN weight makes the sum a NaN)
+        if (!__any(!(top <= 0x1p15f && sum <= 0x1p90f))) {
+            r.l += sum;
+            return 1.f;
+        }
+    }
+    float vm = 0.f, mx = -INFINITY, s[4][4];
     unsigned seen = 0;
 #pragma unroll
-    for (int x = 0; x < 4; x++)
+    for (int x = 0; x < 4; x++) {
+        const f32x4 k = kq(x), v = vs(x);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (FULL) {
-                vm = fmaxf(vm, vs[x][i]);
-            } else {
-                const bool in = sees(co, t + 16 * x + i, len);
-                seen |= (unsigned)in << (4 * x + i);
-                sc[x][i] = in ? sc[x][i] : -INFINITY;
-                vm = fmaxf(vm, in ? vs[x][i] : 0.f);
-            }
-            mx = fmaxf(mx, sc[x][i]);
+            const bool in = full || sees(co, t + 16 * x + i, len);
+            seen |= (unsigned)in << (4 * x + i);
+            s[x][i] = in ? sc[x][i] * k[i] : -INFINITY;
+            vm = fmaxf(vm, in ? v[i] : 0.f);
+            mx = fmaxf(mx, s[x][i]);
         }
-    vm = col_max(vm);
-    mx = fmaxf(r.m, col_max(mx));
-    // 2^e >= the largest scale, e >= -80
-    const float e = fmaxf(r.ve, (float)((int)((__float_as_uint(fmaxf(vm, 0x1p-80f)) + 0x7fffffu) >> 23) - 127 - 14));
-    const float ref = mx == -INFINITY ? 0.f : mx + e;
-    float al = 1.f;
-    if (__any(mx != r.m || e != r.ve)) {
-        al = r.m == -INFINITY ? 0.f : exp2_fast(r.m + r.ve - ref);
-        r.l *= al;
-        r.m = mx;
-        r.ve = e;
     }
+    vm = col_max(vm);
+    r.m = fmaxf(r.m, col_max(mx));
+    // 2^e >= the largest scale * 2^-8, e >= -88
+    r.ve = fmaxf(r.ve, (float)((int)((__float_as_uint(fmaxf(vm, 0x1p-80f)) + 0x7fffffu) >> 23) - 127 - 8));
+    // no score yet: a reference that the first one exceeds
+    const float c = r.m == -INFINITY ? -INFINITY : r.m + r.ve, ref = c == -INFINITY ? 0.f : c;
+    const float al = r.c == -INFINITY ? 0.f : exp2_fast(r.c - ref);
+    r.c = c;
     float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; x++) {
+        const f32x4 v = vs(x);
         float w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float p = exp2_fast(sc[x][i] - ref);
+            const float p = exp2_fast(s[x][i] - ref);
             sum += p;
-            w[i] = p * vs[x][i];
-            if (!FULL && !(seen >> (4 * x + i) & 1)) w[i] = 0.f;  // the scale may be NaN
+            w[i] = seen >> (4 * x + i) & 1 ? p * v[i] : 0.f;  // an unseen scale may be NaN
         }
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 1]));
-            const f16x2 lo = __builtin_bit_cast(
-                f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf(-(float)h[0], 1.f, w[i]), fmaf(-(float)h[1], 1.f, w[i + 1])));
-            wh[x / 2][4 * (x % 2) + i] = h[0];
-            wh[x / 2][4 * (x % 2) + i + 1] = h[1];
-            wl[x / 2][4 * (x % 2) + i] = lo[0];
-            wl[x / 2][4 * (x % 2) + i + 1] = lo[1];
-        }
+        split_weights(w, x, wh, wl);
     }
-    r.l += sum;
+    r.l = r.l * al + sum;
     return al;
 }
 
@@ -376,7 +473,7 @@ __device__ __forceinline__ f16x8 v_operand(int w0, int w1) {
 // Few columns (one tile a workgroup): bound by reading the cache.  Keys go
 // from memory to the operands, every wave with steps of its own.
 template <int KS>
-__global__ __launch_bounds__(64 * WAVES, KS <= 3 ? 2 : 1) void k_tree_i8(TreeArgs a, Kv8Batch cb) {
+__global__ __launch_bounds__(64 * WAVES, KS <= 2 ? 2 : 1) void k_tree_i8(TreeArgs a, Kv8Batch cb) {
     constexpr int DT = 4 * KS, COLS = 16;
     extern __shared__ __align__(16) float sm[];
     Unit u;
@@ -414,30 +511,34 @@ __global__ __launch_bounds__(64 * WAVES, KS <= 3 ? 2 : 1) void k_tree_i8(TreeArg
     for (int st = lo + wave; st < hi; st += WAVES) {
         const int t0 = st * 64;
         const int8_t *vt = vb + (size_t)t0 * hdp;
-        f32x4 vs[4], sc[4];
+        f32x4 vs[4], sc[4], kq[4];
 #pragma unroll
         for (int x = 0; x < 4; x++) vs[x] = *(const f32x4 *)(vsb + t0 + 16 * x + 4 * j);
+        digit_scores<KS, 4>(kk, qd, sc);
 #pragma unroll
-        for (int x = 0; x < 4; x++) sc[x] = digit_scores<KS>(kk[x], qd) * (ks[x] * qs);
+        for (int x = 0; x < 4; x++) kq[x] = ks[x] * qs;
         i32x4 vv[DT];  // K is used up: its registers take V
 #pragma unroll
         for (int d = 0; d < DT; d++)
             vv[d] = 16 * d < hdp ? *(const i32x4 *)(vt + (16 * d + cl) * 64 + 16 * j) : i32x4{0, 0, 0, 0};
         f16x8 wh[2], wl[2];
-        const float al = t0 + 64 <= len ? softmax_step<true>(r, sc, vs, co, t0 + 4 * j, len, wh, wl)
-                                        : softmax_step<false>(r, sc, vs, co, t0 + 4 * j, len, wh, wl);
+        const float al = softmax_step(r, sc, [&](int x) { return kq[x]; }, [&](int x) { return vs[x]; }, t0 + 64 <= len, co, t0 + 4 * j, len, wh, wl);
         if (__any(al != 1.f)) {
 #pragma unroll
             for (int d = 0; d < DT; d++) o[d] *= al;
         }
         load_k(min(st + WAVES, hi - 1));  // under the products below
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int x = 0; x < 2; x++)
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const f16x8 va = v_operand(vv[d][2 * x], vv[d][2 * x + 1]);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wh[x], o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl[x], o[d], 0, 0, 0);
+            for (int d = 0; d < DT; d += 4) {  // four dimensions' products between two of one
+                f16x8 va[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) va[e] = v_operand(vv[d + e][2 * x], vv[d + e][2 * x + 1]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[d + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], wh[x], o[d + e], 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[d + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], wl[x], o[d + e], 0, 0, 0);
             }
     }
 
@@ -445,7 +546,7 @@ __global__ __launch_bounds__(64 * WAVES, KS <= 3 ? 2 : 1) void k_tree_i8(TreeArg
     float *s_o = sm, *s_c = sm + WAVES * COLS * ld, *s_l = s_c + WAVES * COLS;
     const float sum = col_sum(r.l);
     if (j == 0) {
-        s_c[col] = r.m == -INFINITY ? r.m : r.m + r.ve;
+        s_c[col] = r.c;
         s_l[col] = sum;
     }
 #pragma unroll
@@ -459,7 +560,7 @@ __global__ __launch_bounds__(64 * WAVES, KS <= 3 ? 2 : 1) void k_tree_i8(TreeArg
 // a step, V as f16 (converted once for the W tiles), in the order in which the
 // lanes take their operands, and holds the next step's part in registers.
 template <int KS, int W>
-__global__ __launch_bounds__(64 * W, KS == 1 ? 4 : KS == 2 ? 3 : 2) void k_tree_i8_wide(TreeArgs a, Kv8Batch cb) {
+__global__ __launch_bounds__(64 * W, (KS == 1 ? 4 : KS == 2 ? 3 : 2) - (W < 4 ? 1 : 0)) void k_tree_i8_wide(TreeArgs a, Kv8Batch cb) {
     constexpr int DT = 4 * KS, XB = (4 + W - 1) / W, DB = (DT + W - 1) / W;
     __shared__ i32x4 s_k[4][KS][64];
     __shared__ f16x8 s_v[DT][2][64];
@@ -520,30 +621,34 @@ __global__ __launch_bounds__(64 * W, KS == 1 ? 4 : KS == 2 ? 3 : 2) void k_tree_
         __syncthreads();
         fetch(min(st + 1, hi - 1));
         if (t0 >= end) continue;  // (uniform in the wave)
-        f32x4 sc[4], vs[4];
+        f32x4 sc[4];
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-            i32x4 kk[KS];
+        for (int x = 0; x < 4; x += 2) {
+            i32x4 kk[2][KS];
 #pragma unroll
-            for (int k = 0; k < KS; k++) kk[k] = s_k[x][k][lane];
-            sc[x] = digit_scores<KS>(kk, qd) * (s_sc[0][4 * x + j] * qs);
+            for (int k = 0; k < KS; k++) {
+                kk[0][k] = s_k[x][k][lane];
+                kk[1][k] = s_k[x + 1][k][lane];
+            }
+            digit_scores<KS, 2>(kk, qd, sc + x);
         }
-#pragma unroll
-        for (int x = 0; x < 4; x++) vs[x] = s_sc[1][4 * x + j];
         f16x8 wh[2], wl[2];
-        const float al = t0 + 64 <= len ? softmax_step<true>(r, sc, vs, co, t0 + 4 * j, len, wh, wl)
-                                        : softmax_step<false>(r, sc, vs, co, t0 + 4 * j, len, wh, wl);
+        const float al = softmax_step(r, sc, [&](int x) { return s_sc[0][4 * x + j] * qs; }, [&](int x) { return s_sc[1][4 * x + j]; }, t0 + 64 <= len, co, t0 + 4 * j, len, wh, wl);
         if (__any(al != 1.f)) {
 #pragma unroll
             for (int d = 0; d < DT; d++) o[d] *= al;
         }
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int x = 0; x < 2; x++)
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const f16x8 va = s_v[d][x][lane];
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wh[x], o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, wl[x], o[d], 0, 0, 0);
+            for (int d = 0; d < DT; d += 4) {  // four dimensions' products between two of one
+                f16x8 va[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) va[e] = s_v[d + e][x][lane];
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[d + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], wh[x], o[d + e], 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[d + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], wl[x], o[d + e], 0, 0, 0);
             }
     }
 
@@ -560,7 +665,7 @@ __global__ __launch_bounds__(64 * W, KS == 1 ? 4 : KS == 2 ? 3 : 2) void k_tree_
         else
             *(float4 *)(a.part_o + at * hd + dd) = v;
     }
-    if (a.n_split > 1 && j == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(r.m == -INFINITY ? r.m : r.m + r.ve, sum);
+    if (a.n_split > 1 && j == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(r.c, sum);
 }
 
 // ------------------------------------------------------------- f32 cache
@@ -571,36 +676,92 @@ __global__ __launch_bounds__(64 * W, KS == 1 ? 4 : KS == 2 ? 3 : 2) void k_tree_
 // rows 4 j + i as float4 of dimensions 64 e + 4 cl .., so every load is 16
 // bytes wide and a row's lanes are neighbours.
 // ET: blocks of 64 dimensions.
+
+// One step's 16 KB scores of a column (4 KB a lane; key 16 y + 4 j + i at [y][i])
+// into weights; l is rescaled where the reference moves and o's factor returned
+// (1: o stays).
+template <int KB>
+__device__ __forceinline__ float softmax_f32(float &m, float &l, f32x4 (&s)[KB], float scale2, bool full, const Column &co, int t,
+                                             int len, float (&p)[KB][4]) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int y = 0; y < KB; y++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            s[y][i] *= scale2;
+            if (!full) s[y][i] = sees(co, t + 16 * y + i, len) ? s[y][i] : -INFINITY;
+            mx = fmaxf(mx, s[y][i]);
+        }
+    mx = fmaxf(m, col_max(mx));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float al = 1.f;
+    if (__any(mx != m)) {
+        al = m == -INFINITY ? 0.f : exp2_fast(m - ref);
+        l *= al;
+        m = mx;
+    }
+#pragma unroll
+    for (int y = 0; y < KB; y++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            p[y][i] = exp2_fast(s[y][i] - ref);
+            l += p[y][i];
+        }
+    return al;
+}
+
+// Adds the values of V that are not finite, of the keys that the column sees:
+// o[e][f][r] is dimension 64 e + 16 j + 4 r + f.
+template <int ET>
+__device__ __forceinline__ void add_odd(f32x4 (&o)[ET][4], const float (&p)[4], const Column &co, const float *vt, int ldk, int hd, int t0,
+                                        int left, int len) {
+    const int lane = threadIdx.x & 63, cl = lane & 15, j = lane >> 4;
+#pragma unroll 1
+    for (int k = 0; k < 16; k += 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float pk = __shfl(p[i], 4 * k + cl);
+            if (k + i >= left || !sees(co, t0 + k + i, len)) continue;
+#pragma unroll
+            for (int e = 0; e < ET; e++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int d = 64 * e + 16 * j + 4 * r;
+                    if (d >= hd) continue;
+                    const f32x4 v = *(const f32x4 *)(vt + (size_t)(k + i) * ldk + d);
+#pragma unroll
+                    for (int f = 0; f < 4; f++)
+                        if (!isfinite(v[f])) o[e][f][r] += pk * v[f];
+                }
+        }
+    }
+}
+
+// Few columns (one tile a workgroup): bound by reading the cache.
 template <int ET>
 __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeArgs a, F32Batch fb) {
-    constexpr int CT = 4 * ET, COLS = 16, QT = 1;
+    constexpr int CT = 4 * ET, COLS = 16;
     extern __shared__ __align__(16) float sm[];
     Unit u;
     if (!unit_of(a, u)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int cl = lane & 15, j = lane >> 4;
     const int hd = a.hd, len = a.d.len[u.s], ldk = a.n_kv * hd, end = len + a.d.rows;
-
-    const unsigned long long anc = a.d.tree ? ancestor_mask(a.d, u.s) : 0;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    Column co[QT];
-    f32x4 q[QT][CT], o[QT][ET][4];
-    float m[QT], l[QT];
+    const int c = u.qg * COLS + cl;
+    const Column co = column_of(a, u.s, c, a.d.tree ? ancestor_mask(a.d, u.s) : 0);
+    f32x4 q[CT], o[ET][4];
+    {
+        const int cc = min(c, a.cols - 1);
+        const float *qr = a.q + (((size_t)u.s * a.d.rows + cc / a.nrep) * a.n_q + u.g * a.nrep + cc % a.nrep) * hd;
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const int c = u.qg * COLS + 16 * t + cl;
-        co[t] = column_of(a, u.s, c, anc);
-        const int node = min(c, a.cols - 1) / a.nrep, rep = min(c, a.cols - 1) % a.nrep;
-        const float *qr = a.q + (((size_t)u.s * a.d.rows + node) * a.n_q + u.g * a.nrep + rep) * hd;
-#pragma unroll
-        for (int x = 0; x < CT; x++) q[t][x] = 16 * x + 4 * j < hd ? *(const f32x4 *)(qr + 16 * x + 4 * j) : zero;
-#pragma unroll
-        for (int e = 0; e < ET; e++)
-#pragma unroll
-            for (int f = 0; f < 4; f++) o[t][e][f] = zero;
-        m[t] = -INFINITY;
-        l[t] = 0.f;
+        for (int x = 0; x < CT; x++) q[x] = 16 * x + 4 * j < hd ? *(const f32x4 *)(qr + 16 * x + 4 * j) : zero;
     }
+#pragma unroll
+    for (int e = 0; e < ET; e++)
+#pragma unroll
+        for (int f = 0; f < 4; f++) o[e][f] = zero;
+    float m = -INFINITY, l = 0.f;
     const float *kb = fb.k[u.s] + (size_t)u.g * hd, *vb = fb.v[u.s] + (size_t)u.g * hd;
     int lo, hi;
     step_range<16>(a, u, COLS, &lo, &hi);
@@ -623,146 +784,251 @@ __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeAr
 #pragma unroll
             for (int e = 0; e < ET; e++)
                 vv[i][e] = 4 * j + i < left && 64 * e + 4 * cl < hd ? *(const f32x4 *)(vt + (size_t)(4 * j + i) * ldk + 64 * e + 4 * cl) : zero;
-
+        f32x4 s0 = zero, s1 = zero;
+#pragma unroll
+        for (int x = 0; x < CT; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[x][e], q[x][e], s0, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[x][e + 1], q[x][e + 1], s1, 0, 0, 0);
+            }
+        load_k(min(st + WAVES, hi - 1));  // K is used up: under the products p.v
         const bool full = t0 + 16 <= len;
+        // In drafted rows a value that is not finite may be seen by one column
+        // and not by another: 0 * inf must not reach the latter.  Such values
+        // leave the products here and are added one by one below.
         bool odd = false;
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-            f32x4 s0 = zero, s1 = zero;
-#pragma unroll
-            for (int x = 0; x < CT; x++) {
-                if (16 * x < hd)
-#pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[x][e], q[t][x][e], s0, 0, 0, 0);
-                    s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[x][e + 1], q[t][x][e + 1], s1, 0, 0, 0);
-                }
-            }
-            if (t == QT - 1) load_k(min(st + WAVES, hi - 1));  // K is used up: under the products p.v
-            // In drafted rows a value that is not finite may be seen by one column
-            // and not by another: 0 * inf must not reach the latter.  Such values
-            // leave the products here and are added one by one below.
-            if (!full && t == 0) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int e = 0; e < ET; e++)
-#pragma unroll
-                        for (int f = 0; f < 4; f++)
-                            if (!isfinite(vv[i][e][f])) {
-                                odd = true;
-                                vv[i][e][f] = 0.f;
-                            }
-                odd = __any(odd);
-            }
-            float sc[4];
-            float mx = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                sc[i] = (s0[i] + s1[i]) * a.scale2;
-                if (!full) sc[i] = sees(co[t], t0 + 4 * j + i, len) ? sc[i] : -INFINITY;
-                mx = fmaxf(mx, sc[i]);
-            }
-            mx = fmaxf(m[t], col_max(mx));
-            const float ref = mx == -INFINITY ? 0.f : mx;
-            if (__any(mx != m[t])) {
-                const float al = m[t] == -INFINITY ? 0.f : exp2_fast(m[t] - ref);
-                l[t] *= al;
-#pragma unroll
-                for (int e = 0; e < ET; e++)
-#pragma unroll
-                    for (int f = 0; f < 4; f++) o[t][e][f] *= al;
-                m[t] = mx;
-            }
-            float p[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                p[i] = exp2_fast(sc[i] - ref);
-                l[t] += p[i];
-            }
+        if (!full) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int e = 0; e < ET; e++)
 #pragma unroll
                     for (int f = 0; f < 4; f++)
-                        o[t][e][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[i][e][f], p[i], o[t][e][f], 0, 0, 0);
-            if (odd) {
-                // o[e][f][r] is dimension 64 e + 16 j + 4 r + f of column cl
-#pragma unroll 1
-                for (int k = 0; k < 16; k += 4) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float pk = __shfl(p[i], 4 * k + cl);
-                        if (k + i >= left || !sees(co[t], t0 + k + i, len)) continue;
-#pragma unroll
-                        for (int e = 0; e < ET; e++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++) {
-                                const int d = 64 * e + 16 * j + 4 * r;
-                                const f32x4 v = d < hd ? *(const f32x4 *)(vt + (size_t)(k + i) * ldk + d) : zero;
-#pragma unroll
-                                for (int f = 0; f < 4; f++)
-                                    if (!isfinite(v[f])) o[t][e][f][r] += pk * v[f];
-                            }
-                    }
-                }
-            }
+                        if (!isfinite(vv[i][e][f])) {
+                            odd = true;
+                            vv[i][e][f] = 0.f;
+                        }
+            odd = __any(odd);
         }
+        float p[1][4];
+        f32x4 sc[1] = {s0 + s1};
+        const float al = softmax_f32<1>(m, l, sc, a.scale2, full, co, t0 + 4 * j, len, p);
+        if (__any(al != 1.f)) {
+#pragma unroll
+            for (int e = 0; e < ET; e++)
+#pragma unroll
+                for (int f = 0; f < 4; f++) o[e][f] *= al;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < ET; e++)
+#pragma unroll
+                for (int f = 0; f < 4; f++) o[e][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[i][e][f], p[0][i], o[e][f], 0, 0, 0);
+        if (odd) add_odd<ET>(o, p[0], co, vt, ldk, hd, t0, left, len);
     }
 
-    const int ld = hd + 4;
+    const int ld = hd + 4, col = wave * COLS + cl;
     float *s_o = sm, *s_c = sm + WAVES * COLS * ld, *s_l = s_c + WAVES * COLS;
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const int col = wave * COLS + 16 * t + cl;
-        const float sum = col_sum(l[t]);
-        if (j == 0) {
-            s_c[col] = m[t];
-            s_l[col] = sum;
-        }
-#pragma unroll
-        for (int e = 0; e < ET; e++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int d = 64 * e + 16 * j + 4 * r;
-                if (d < hd) *(f32x4 *)(s_o + col * ld + d) = f32x4{o[t][e][0][r], o[t][e][1][r], o[t][e][2][r], o[t][e][3][r]};
-            }
+    const float sum = col_sum(l);
+    if (j == 0) {
+        s_c[col] = m;
+        s_l[col] = sum;
     }
+#pragma unroll
+    for (int e = 0; e < ET; e++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int d = 64 * e + 16 * j + 4 * r;
+            if (d < hd) *(f32x4 *)(s_o + col * ld + d) = f32x4{o[e][0][r], o[e][1][r], o[e][2][r], o[e][3][r]};
+        }
     join_waves<COLS>(a, u, s_o, s_c, s_l, ld);
 }
 
-// Key splits: about `want` workgroups, each with at least `least` steps.
-int pick_splits(const TreeArgs &a, int step_keys, int want, int least) {
-    int len = 0;
-    for (int s = 0; s < a.d.n_seq; s++) len = len > a.d.len[s] ? len : a.d.len[s];
-    const long long steps = ((long long)len + a.d.rows + step_keys - 1) / step_keys;
-    const long long units = (long long)a.d.n_seq * a.n_kv * a.n_qg;
-    long long n = (want + units - 1) / units;
-    const long long most = steps / least;
-    if (n > most) n = most;
-    if (n > MAX_SPLIT) n = MAX_SPLIT;
-    return n < 1 ? 1 : (int)n;
+// Many columns: bound by the f32 matrix rate.  W waves with a tile each share
+// a step's keys through LDS, in operand order; the next step's part waits in
+// registers.  A step is 16 keys, 32 where heads are short (at 128 dimensions 32
+// keys a step left fewer waves: 26-node trees of four contexts 62 against 56 us).
+constexpr int tree_f32_blocks(int et) { return et == 1 ? 2 : 1; }
+template <int ET, int W>
+__global__ __launch_bounds__(64 * W, ET <= 2 ? 3 : ET == 4 && W == 2 ? 1 : 2) void k_tree_f32_wide(TreeArgs a, F32Batch fb) {
+    constexpr int CT = 4 * ET, KB = tree_f32_blocks(ET), NB = (KB * CT + W - 1) / W;
+    __shared__ f32x4 s_k[KB * CT][64], s_v[KB * CT][64];  // block y, x: [y CT + x]; V's x = i ET + e
+    __shared__ int s_odd[W];
+    Unit u;
+    if (!unit_of(a, u)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cl = lane & 15, j = lane >> 4;
+    const int hd = a.hd, len = a.d.len[u.s], ldk = a.n_kv * hd, rows_end = len + a.d.rows;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const int c0 = (u.qg * W + wave) * 16, c = c0 + cl;
+    const Column co = column_of(a, u.s, c, a.d.tree ? ancestor_mask(a.d, u.s) : 0);
+    const int end = c0 >= a.cols ? 0 : a.d.tree ? rows_end : len + min(c0 + 15, a.cols - 1) / a.nrep + 1;
+    f32x4 q[CT], o[ET][4];
+    {
+        const int cc = min(c, a.cols - 1);
+        const float *qr = a.q + (((size_t)u.s * a.d.rows + cc / a.nrep) * a.n_q + u.g * a.nrep + cc % a.nrep) * hd;
+#pragma unroll
+        for (int x = 0; x < CT; x++) q[x] = 16 * x + 4 * j < hd ? *(const f32x4 *)(qr + 16 * x + 4 * j) : zero;
+    }
+#pragma unroll
+    for (int e = 0; e < ET; e++)
+#pragma unroll
+        for (int f = 0; f < 4; f++) o[e][f] = zero;
+    float m = -INFINITY, l = 0.f;
+    const float *kb = fb.k[u.s] + (size_t)u.g * hd, *vb = fb.v[u.s] + (size_t)u.g * hd;
+    int lo, hi;
+    step_range<16 * KB>(a, u, 16 * W, &lo, &hi);
+
+    f32x4 kr[NB], vr[NB];
+    auto fetch = [&](int st) {
+        const float *kt = kb + (size_t)st * 16 * KB * ldk, *vt = vb + (size_t)st * 16 * KB * ldk;
+        const int left = rows_end - st * 16 * KB;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const int y = (W * b + wave) / CT, x = (W * b + wave) % CT, i = x / ET, e = x % ET;
+            const int rk = 16 * y + cl, rv = 16 * y + 4 * j + i;
+            const bool in = W * b + wave < KB * CT;
+            kr[b] = in && rk < left && 16 * x + 4 * j < hd ? *(const f32x4 *)(kt + (size_t)rk * ldk + 16 * x + 4 * j) : zero;
+            vr[b] = in && rv < left && 64 * e + 4 * cl < hd ? *(const f32x4 *)(vt + (size_t)rv * ldk + 64 * e + 4 * cl) : zero;
+        }
+    };
+    if (lo < hi) fetch(lo);
+    for (int st = lo; st < hi; st++) {
+        const int t0 = st * 16 * KB;
+        const bool full = t0 + 16 * KB <= len;
+        bool odd = false;
+        if (!full) {  // values that are not finite leave the products, as in k_tree_f32
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int f = 0; f < 4; f++)
+                    if (!isfinite(vr[b][f])) {
+                        odd = true;
+                        vr[b][f] = 0.f;
+                    }
+            odd = __any(odd);
+        }
+        __syncthreads();  // the step before has been read
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+            if (W * b + wave < KB * CT) {
+                s_k[W * b + wave][lane] = kr[b];
+                s_v[W * b + wave][lane] = vr[b];
+            }
+        if (lane == 0) s_odd[wave] = odd;
+        __syncthreads();
+        fetch(min(st + 1, hi - 1));
+        if (t0 >= end) continue;  // (uniform in the wave)
+        f32x4 s0[KB], s1[KB];
+#pragma unroll
+        for (int y = 0; y < KB; y++) s0[y] = s1[y] = zero;
+#pragma unroll
+        for (int x = 0; x < CT; x++)
+#pragma unroll
+            for (int y = 0; y < KB; y++) {
+                const f32x4 kk = s_k[y * CT + x][lane];
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    s0[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], q[x][e], s0[y], 0, 0, 0);
+                    s1[y] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e + 1], q[x][e + 1], s1[y], 0, 0, 0);
+                }
+            }
+        float p[KB][4];
+        f32x4 sc[KB];
+#pragma unroll
+        for (int y = 0; y < KB; y++) sc[y] = s0[y] + s1[y];
+        const float al = softmax_f32<KB>(m, l, sc, a.scale2, full, co, t0 + 4 * j, len, p);
+        if (__any(al != 1.f)) {
+#pragma unroll
+            for (int e = 0; e < ET; e++)
+#pragma unroll
+                for (int f = 0; f < 4; f++) o[e][f] *= al;
+        }
+#pragma unroll
+        for (int y = 0; y < KB; y++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < ET; e++) {
+                    const f32x4 vv = s_v[y * CT + i * ET + e][lane];
+#pragma unroll
+                    for (int f = 0; f < 4; f++) o[e][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[f], p[y][i], o[e][f], 0, 0, 0);
+                }
+        if (!full) {
+            int any = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++) any |= s_odd[w];
+            if (any)
+#pragma unroll
+                for (int y = 0; y < KB; y++)
+                    add_odd<ET>(o, p[y], co, vb + ((size_t)t0 + 16 * y) * ldk, ldk, hd, t0 + 16 * y, rows_end - t0 - 16 * y, len);
+        }
+    }
+
+    const float sum = col_sum(l), inv = 1.f / sum;
+    if (c >= a.cols) return;
+    const size_t at = part_of(a, u, c);
+#pragma unroll
+    for (int e = 0; e < ET; e++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int d = 64 * e + 16 * j + 4 * r;
+            if (d >= hd) continue;
+            const float4 v = make_float4(o[e][0][r], o[e][1][r], o[e][2][r], o[e][3][r]);
+            if (a.n_split == 1)
+                store_out(a, u.s, u.g, c, d, v, inv);
+            else
+                *(float4 *)(a.part_o + at * hd + d) = v;
+        }
+    if (a.n_split > 1 && j == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(m, sum);
+}
+
+// Key splits: about `want` workgroups in all, each of `least` steps or more,
+// the sequences' splits of like sizes.
+void pick_splits(TreeArgs &a, int step_keys, int want, int least) {
+    long long steps[PF_MAX_SEQS], all = 0;
+    for (int s = 0; s < a.d.n_seq; s++) all += steps[s] = ((long long)a.d.len[s] + a.d.rows + step_keys - 1) / step_keys;
+    long long size = (all * a.n_kv * a.n_qg + want - 1) / want;
+    if (size < least) size = least;
+    a.n_split = 1;
+    for (int s = 0; s < a.d.n_seq; s++) {
+        long long n = (steps[s] + size / 2) / size;
+        n = n < 1 ? 1 : n > MAX_SPLIT ? MAX_SPLIT : n;
+        a.splits[s] = (int)n;
+        if (a.n_split < n) a.n_split = (int)n;
+    }
 }
 
 // waves: of a workgroup; cols: its columns
 template <class K, class B>
 int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t lds, int step_keys, int want, int least, hipStream_t s) {
     a.n_qg = (a.cols + cols - 1) / cols;
-    a.n_split = pick_splits(a, step_keys, want, least);
+    pick_splits(a, step_keys, want, least);
     const size_t n_col = (size_t)a.d.n_seq * a.n_kv * a.cols;
     void *ws = nullptr;
     SCRY_TRY(split_workspace(n_col * (a.hd + 2) * sizeof(float), &a.n_split, &ws));
     a.part_o = (float *)ws;
     a.part_ml = a.part_o + n_col * a.n_split * a.hd;
-    a.n_pair = a.d.n_seq * a.n_kv * a.n_split;
-    const size_t grid = (size_t)((a.n_pair + 7) / 8) * 8 * a.n_qg;
+    for (int i = 0; i < a.d.n_seq; i++) {
+        if (a.n_split == 1) a.splits[i] = 1;  // one is enough, or no memory for more
+        a.pair0[i + 1] = a.pair0[i] + a.n_kv * a.splits[i];
+    }
+    const size_t grid = (size_t)((a.pair0[a.d.n_seq] + 7) / 8) * 8 * a.n_qg;
     if (grid > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "attention: %zu workgroups", grid);
     if (lds > 65536)
         SCRY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), lds, s, a, b);
     SCRY_HIP(hipGetLastError());
-    if (a.n_split > 1) {
+    // a thread per four dimensions where they fill the chip, else the groups of
+    // k_tree_merge (16384 columns of 128 by 3 splits: 8 against 13 us; 32 by 64:
+    // 4 against MERGEFLAT us)
+    const size_t n = n_col * (a.hd / 4);
+    if (a.n_split > 1 && n >= (size_t)1 << 15) {
+        hipLaunchKernelGGL(k_tree_merge_flat, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, n);
+        SCRY_HIP(hipGetLastError());
+    } else if (a.n_split > 1) {
         int lanes = 1;
         while (4 * lanes < a.hd) lanes *= 2;
         // threads of a column: its lanes, times up to as many groups as it has splits
@@ -782,6 +1048,8 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
 #define LEASTW 4
 #define WANTF 768
 #define LEASTF 8
+#define WANTFW 768
+#define LEASTFW 4
 #endif
 template <int KS>
 int launch_i8(const TreeArgs &a, const Kv8Batch &b, hipStream_t s) {
@@ -794,8 +1062,12 @@ int launch_i8(const TreeArgs &a, const Kv8Batch &b, hipStream_t s) {
 }
 template <int ET>
 int launch_f32(const TreeArgs &a, const F32Batch &b, hipStream_t s) {
+    const int tiles = (a.cols + 15) / 16, groups = (tiles + 3) / 4, w = (tiles + groups - 1) / groups;
     const size_t lds = (size_t)WAVES * 16 * (a.hd + 4 + 2) * sizeof(float);
-    return launch_tree(k_tree_f32<ET>, a, b, WAVES, 16, lds, 16, WANTF, LEASTF, s);
+    if (w == 1) return launch_tree(k_tree_f32<ET>, a, b, WAVES, 16, lds, 16, WANTF, LEASTF, s);
+    if (w == 2) return launch_tree(k_tree_f32_wide<ET, 2>, a, b, 2, 32, 0, 16 * tree_f32_blocks(ET), 2 * WANTFW, LEASTFW, s);
+    if (w == 3) return launch_tree(k_tree_f32_wide<ET, 3>, a, b, 3, 48, 0, 16 * tree_f32_blocks(ET), 4 * WANTFW / 3, LEASTFW, s);
+    return launch_tree(k_tree_f32_wide<ET, 4>, a, b, 4, 64, 0, 16 * tree_f32_blocks(ET), WANTFW, LEASTFW, s);
 }
 
 int tree_run(const char *what, scry_buf q, const TreeArgs &t, bool i8, const F32Batch &f, const Kv8Batch &c, scry_buf *out) {
