@@ -418,6 +418,7 @@ int scry_hip_shutdown(void) {
     if (!c.init) return SCRY_OK;
     (void)hipStreamSynchronize(c.stream);
     host_block_free();
+    verify_free();
     pool_trim();
     dev_free(c.ws);
     (void)hipStreamDestroy(c.stream);

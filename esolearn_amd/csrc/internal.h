@@ -469,6 +469,7 @@ int check_heads(const char *what, int n_q, int n_kv, int head_dim);  // n_q = 0:
 // for the stream before they return
 int host_block(size_t bytes, void **p);
 void host_block_free();
+void verify_free();  // verify.hip: its counters
 
 // bf16.hip -- bf16 mode: the reference's cast, widening, B-operand rows
 // [n][kp] (kp = bf16_row_pad(k)), the GEMM activation plane, the bf16 GEMV

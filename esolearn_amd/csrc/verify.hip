@@ -14,9 +14,12 @@
 // f64.  Weights that are not positive and finite count as zero; where none is
 // left, the residual falls back to p, and p to equal weights.
 //
-// The row is cut into chunks summed by a workgroup each; then one workgroup
-// finds the chunk, and in it the token.  Bound by latency, and for trees by
-// reading their rows once.
+// One launch.  A row is cut into chunks, a workgroup each, whose four waves
+// leave the sums of their parts; the last workgroup of a row to arrive finds
+// the part, and in it the token; for a tree, the last row of a sequence walks.
+// A chain reads one row of p (and of q) of a sequence and is bound by the
+// latency of that sequence of steps; a tree reads its rows once, at the rate of
+// the memory.
 #include <cmath>
 #include <cstring>
 
@@ -29,7 +32,6 @@ namespace {
 using namespace dev;
 
 constexpr int VF_MAX_ROWS = DRAFT_MAX_TREE;  // drafted tokens of a sequence
-constexpr int VF_MAX_CHUNKS = 1024;
 constexpr int VF_ARGS = 160;  // (token, number) pairs that travel in the kernel's arguments
 
 struct VfIn {  // n_seq * (rows + 1) of each: a sequence's tokens (the last place unused) and its numbers
@@ -39,31 +41,61 @@ struct VfIn {  // n_seq * (rows + 1) of each: a sequence's tokens (the last plac
 
 struct VfArgs {
     const float *p, *q;  // [n_seq][rows + 1][V]; [n_seq][rows][V], null for a tree
-    int V, rows, chunk, n_chunk, tree;
+    int V, rows, sub, n_sub, tree, wide;  // sub: values of a wave's part; wide: rows are 16-byte aligned
     signed char count[PF_MAX_SEQS];
-    double *part;  // [n_seq][R][2][n_chunk]: sums of the weights and of p; R = rows + 1 (tree) or 1
-    int *drawn;    // tree: [n_seq][rows + 1]
-    int *out;      // pinned, [n_seq][2 + rows]: accepted, next token, path
-    const double *u;  // null: in the arguments, with the tokens
+    double *part;       // [n_seq][R][2][n_sub]: sums of the weights and of p; R = rows + 1 (tree) or 1
+    int *drawn;         // tree: [n_seq][rows + 1]
+    unsigned *arrived;  // [n_seq][VF_MAX_ROWS + 2]: workgroups per row, rows per sequence; zero between launches
+    int *out;           // pinned, [n_seq][2 + rows]: accepted, next token, path
+    const double *u;    // null: in the arguments, with the tokens
     const int *tok;
 };
 __device__ __forceinline__ const double *vf_u(const VfArgs &a, const VfIn &in) { return a.u ? a.u : in.u; }
 __device__ __forceinline__ const int *vf_tok(const VfArgs &a, const VfIn &in) { return a.u ? a.tok : in.tok; }
 
+__device__ __forceinline__ double weight(float p) { return p > 0.f && p < INFINITY ? (double)p : 0.0; }
 __device__ __forceinline__ double weight(float p, float q) {
     const double w = (double)p - (double)q;
     return w > 0.0 && w < (double)INFINITY ? w : 0.0;
 }
 
-// What sequence s draws from: row r of p, less row r of q where less is set.
+// Values that other workgroups, on other XCDs, read in this launch: device-scope
+// accesses go past the XCD's own L2.
+template <class T>
+__device__ __forceinline__ void put(T *p, T v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class T>
+__device__ __forceinline__ T get(const T *p) {
+    return __hip_atomic_load(const_cast<T *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// With every thread of the workgroup: whether it is the last of n to arrive.
+// What the others put before they arrived, it gets: each wave waits until its
+// device-scope stores are complete, then the barrier, then the count.  (A
+// release fence would write back the XCD's whole L2, once a workgroup: 16
+// sequences at V = 128256 took 91 us with it.)
+__device__ __forceinline__ bool last_to_arrive(unsigned *ctr, unsigned n) {
+    __shared__ int s_last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s_last = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+        if (s_last) put(ctr, 0u);  // for the next launch
+    }
+    __syncthreads();
+    return s_last;
+}
+
+// What sequence s draws from: row p, less row q where it is set.  For a chain
+// every wave looks at all of the sequence's tokens, one a lane.
 struct VfRow {
     const float *p, *q;
-    int r;
+    int n;  // chain: accepted
 };
-__device__ __forceinline__ VfRow vf_row(const VfArgs &a, const VfIn &in, int s, int r, int *n_ok) {
+__device__ __forceinline__ VfRow vf_row(const VfArgs &a, const VfIn &in, int s, int r) {
     const size_t V = a.V;
     const float *p = a.p + (size_t)s * (a.rows + 1) * V;
-    if (a.tree) return {p + r * V, nullptr, r};
+    if (a.tree) return {p + r * V, nullptr, 0};
     const int n = a.count[s], lane = threadIdx.x & 63, at = s * (a.rows + 1) + lane;
     bool ok = true;
     if (lane < n) {
@@ -72,147 +104,99 @@ __device__ __forceinline__ VfRow vf_row(const VfArgs &a, const VfIn &in, int s, 
     }
     const unsigned long long no = __ballot(!ok);
     const int k = no ? __ffsll((long long)no) - 1 : n;
-    *n_ok = k;
     return {p + k * V, k < n ? a.q + ((size_t)s * a.rows + k) * V : nullptr, k};
 }
 
-__device__ __forceinline__ double block_sum(double v, double *red) {
-    v = wave_sum_d(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
-}
-
-__global__ __launch_bounds__(256) void k_verify_sums(VfArgs a, VfIn args) {
-    __shared__ double red[4];
-    const int s = blockIdx.z, r = blockIdx.y, c = blockIdx.x;
-    int n = 0;
-    const VfRow w = vf_row(a, args, s, r, &n);
-    const int lo = c * a.chunk, hi = min(a.V, lo + a.chunk);
-    double sw = 0.0, sp = 0.0;
-    for (int j = lo + (int)threadIdx.x; j < hi; j += 256) {
-        sp += weight(w.p[j], 0.f);
-        if (w.q) sw += weight(w.p[j], w.q[j]);
-    }
-    sp = block_sum(sp, red);
-    if (w.q) sw = block_sum(sw, red);
-    if (threadIdx.x == 0) {
-        double *d = a.part + (((size_t)s * gridDim.y + r) * 2) * a.n_chunk + c;
-        d[0] = w.q ? sw : sp;
-        d[a.n_chunk] = sp;
-    }
-}
-
-// Inclusive running sums over the workgroup's threads.
-__device__ __forceinline__ double block_scan(double v, double *red) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Inclusive running sums over the wave's lanes.
+__device__ __forceinline__ double wave_scan(double v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const double o = __shfl_up(v, off);
         if (lane >= off) v += o;
     }
-    __syncthreads();
-    if (lane == 63) red[wave] = v;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) v += red[w];
     return v;
 }
 
-// The lowest i in [0, n) with f(i) > 0 whose running sum of f, from `base` on,
-// passes target; where rounding leaves none, the last i with f(i) > 0 (-1: no
-// such i).  A thread takes ceil(n / 256) neighbours; the first thread whose end
-// passes looks through its own.  *before: the running sum below i.
-template <class F>
-__device__ __forceinline__ int block_find(int n, double target, double base, F f, double *before, double *red) {
-    __shared__ double s_end[256], s_before;
-    __shared__ int s_first, s_last, s_i;
-    const int tid = threadIdx.x, per = (n + 255) / 256, lo = min(n, tid * per), hi = min(n, lo + per);
-    if (tid == 0) {
-        s_first = 256;
-        s_last = s_i = -1;
-        s_before = base;
-    }
-    double own = 0.0;
-    for (int i = lo; i < hi; i++) own += f(i);
-    const double end = base + block_scan(own, red);  // (barriers: the shared values above are set)
-    s_end[tid] = end;
-    if (own > 0.0) {
-        if (end > target) atomicMin(&s_first, tid);
-        atomicMax(&s_last, tid);
-    }
-    __syncthreads();
-    if (tid == (s_first < 256 ? s_first : s_last)) {
-        double x = tid ? s_end[tid - 1] : base;
-        for (int i = lo; i < hi; i++) {
-            const double w = f(i);
-            if (!(w > 0.0)) continue;
-            s_i = i;
-            s_before = x;
-            x += w;
-            if (x > target) break;
+// One wave: the lowest i in [lo, hi) with f(i) > 0 whose running sum of f, from
+// `base` on, passes target; where rounding leaves none, the last with f(i) > 0
+// (-1: no such i).  *base: the running sum below that i.  A lane takes PER
+// neighbours of 64 PER at a time.
+template <int PER, class F>
+__device__ __forceinline__ int wave_find(int lo, int hi, double target, double *base, F f) {
+    const int lane = threadIdx.x & 63;
+    int last = -1;
+    double below = *base, run = *base;  // below: the sum below `last`
+    for (int i0 = lo; i0 < hi; i0 += 64 * PER) {
+        double w[PER], own = 0.0;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            const int i = i0 + lane * PER + k;
+            w[k] = i < hi ? f(i) : 0.0;
+            own += w[k];
         }
+        const double end = run + wave_scan(own);
+        const double prev = __shfl_up(end, 1);
+        const unsigned long long some = __ballot(own > 0.0), pass = __ballot(own > 0.0 && end > target);
+        if (some) {
+            const int who = pass ? __ffsll((long long)pass) - 1 : 63 - __clzll((long long)some);
+            // that lane looks through its own
+            double x = lane ? prev : run, at = x;
+            int mine = -1;
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                if (!(w[k] > 0.0) || (mine >= 0 && x > target)) continue;
+                mine = i0 + lane * PER + k;
+                at = x;
+                x += w[k];
+            }
+            last = __shfl(mine, who);
+            below = __shfl(at, who);
+            if (pass) break;
+        }
+        run = __shfl(end, 63);
     }
-    __syncthreads();
-    *before = s_before;
-    const int r = s_i;
-    __syncthreads();
-    return r;
+    *base = below;
+    return last;
 }
 
-// The drawn index of sequence s, row r, in every thread.
-__device__ __forceinline__ int vf_draw(const VfArgs &a, const VfRow &w, const double *part, double u, double *red) {
-    double total = 0.0;
+// The index drawn from a row by the first wave of the workgroup, from the sums
+// of its parts.
+__device__ __forceinline__ int vf_draw(const VfArgs &a, const VfRow &w, const double *part, double u) {
+    const int lane = threadIdx.x & 63;
     const float *q = w.q;
-    for (int c = threadIdx.x; c < a.n_chunk; c += 256) total += part[c];
-    total = block_sum(total, red);
-    if (!(total > 0.0)) {  // no residual: p itself
-        q = nullptr;
-        part += a.n_chunk;
+    double total = 0.0;
+    for (int turn = 0; turn < 2; turn++) {
+        for (int c = lane; c < a.n_sub; c += 64) total += get(part + c);
+        total = wave_sum_d(total);
+        if (total > 0.0) break;
+        if (turn || !q) return min(a.V - 1, (int)(u * (double)a.V));  // no mass at all
+        q = nullptr;  // no residual: p itself
+        part += a.n_sub;
         total = 0.0;
-        for (int c = threadIdx.x; c < a.n_chunk; c += 256) total += part[c];
-        total = block_sum(total, red);
-        if (!(total > 0.0)) return min(a.V - 1, (int)(u * (double)a.V));
     }
     const double target = u * total;
-    double before = 0.0;
-    const int c = block_find(a.n_chunk, target, 0.0, [&](int i) { return part[i]; }, &before, red);
-    const int lo = c * a.chunk, n = min(a.chunk, a.V - lo);
-    __syncthreads();
-    double unused;
-    const int j = block_find(n, target, before, [&](int i) { return weight(w.p[lo + i], q ? q[lo + i] : 0.f); }, &unused, red);
-    return lo + max(j, 0);
+    double base = 0.0;
+    const int c = wave_find<4>(0, a.n_sub, target, &base, [&](int i) { return get(part + i); });
+    const int lo = max(c, 0) * a.sub, hi = min(a.V, lo + a.sub);
+    const int j = wave_find<8>(lo, hi, target, &base, [&](int i) { return q ? weight(w.p[i], q[i]) : weight(w.p[i]); });
+    return max(j, 0);
 }
 
-__global__ __launch_bounds__(256) void k_verify_draw(VfArgs a, VfIn args) {
-    __shared__ double red[4];
-    const int s = blockIdx.z, r = blockIdx.y;
-    int n = 0;
-    const VfRow w = vf_row(a, args, s, r, &n);
-    const double *part = a.part + (((size_t)s * gridDim.y + r) * 2) * a.n_chunk;
-    const int j = vf_draw(a, w, part, vf_u(a, args)[s * (a.rows + 1) + (a.tree ? r : a.rows)], red);
-    if (threadIdx.x) return;
-    if (a.tree) {
-        a.drawn[s * (a.rows + 1) + r] = j;
-    } else {
-        a.out[s * (2 + a.rows)] = n;
-        a.out[s * (2 + a.rows) + 1] = j;
-    }
-}
-
-// One wave per sequence, a node per lane.
-__global__ __launch_bounds__(64) void k_verify_walk(VfArgs a, VfIn args, DraftBatch d) {
-    const int s = blockIdx.x, i = threadIdx.x;
+// From row 0 to the child that holds the row's token, a node per lane.
+__device__ __forceinline__ void vf_walk(const VfArgs &a, const VfIn &in, const DraftBatch &d, int s) {
+    const int i = threadIdx.x & 63;
     const int parent = i < a.rows ? (int)d.parent[s][i] : -2;
-    const int tok = i < a.rows ? vf_tok(a, args)[s * (a.rows + 1) + i] : 0;
+    const int tok = i < a.rows ? vf_tok(a, in)[s * (a.rows + 1) + i] : 0;
+    const int t_row = i < a.rows ? get(a.drawn + s * (a.rows + 1) + 1 + i) : 0;  // drawn after node i
     int *out = a.out + s * (2 + a.rows);
-    int cur = -1, n = 0, t;
+    int cur = -1, n = 0, t = get(a.drawn + s * (a.rows + 1));
     for (;;) {
-        t = a.drawn[s * (a.rows + 1) + cur + 1];
         const unsigned long long hit = __ballot(parent == cur && tok == t);
         if (!hit) break;
         cur = __ffsll((long long)hit) - 1;  // above the last one: at most `rows` turns
         if (i == 0) out[2 + n] = cur;
+        t = __shfl(t_row, cur);
         n++;
     }
     if (i >= n && i < a.rows) out[2 + i] = -1;
@@ -222,11 +206,71 @@ __global__ __launch_bounds__(64) void k_verify_walk(VfArgs a, VfIn args, DraftBa
     }
 }
 
+__global__ __launch_bounds__(256) void k_verify(VfArgs a, VfIn in, DraftBatch d) {
+    const int s = blockIdx.z, r = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const VfRow w = vf_row(a, in, s, r);
+    const int c = blockIdx.x * 4 + wave;
+    double *part = a.part + (((size_t)s * gridDim.y + r) * 2) * a.n_sub;
+    if (c < a.n_sub) {
+        const int lo = c * a.sub, hi = min(a.V, lo + a.sub);
+        double sw = 0.0, sp = 0.0;
+        auto add = [&](float p, float q) {
+            sp += weight(p);
+            if (w.q) sw += weight(p, q);
+        };
+        if (a.wide) {
+#pragma unroll 4
+            for (int j = lo + 4 * lane; j < hi; j += 256) {
+                const float4 p = *(const float4 *)(w.p + j);
+                const float4 q = w.q ? *(const float4 *)(w.q + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                add(p.x, q.x);
+                add(p.y, q.y);
+                add(p.z, q.z);
+                add(p.w, q.w);
+            }
+        } else {
+#pragma unroll 8
+            for (int j = lo + lane; j < hi; j += 64) add(w.p[j], w.q ? w.q[j] : 0.f);
+        }
+        sp = wave_sum_d_dpp(sp);
+        sw = w.q ? wave_sum_d_dpp(sw) : sp;
+        if (lane == 0) {
+            put(part + c, sw);
+            put(part + a.n_sub + c, sp);
+        }
+    }
+    unsigned *arrived = a.arrived + s * (VF_MAX_ROWS + 2);
+    if (!last_to_arrive(arrived + 1 + r, gridDim.x)) return;
+    if (wave == 0) {
+        const int j = vf_draw(a, w, part, vf_u(a, in)[s * (a.rows + 1) + (a.tree ? r : a.rows)]);
+        if (lane == 0) {
+            if (a.tree) {
+                put(a.drawn + s * (a.rows + 1) + r, j);
+            } else {
+                a.out[s * (2 + a.rows)] = w.n;
+                a.out[s * (2 + a.rows) + 1] = j;
+            }
+        }
+    }
+    if (!a.tree || !last_to_arrive(arrived, gridDim.y)) return;
+    if (wave == 0) vf_walk(a, in, d, s);
+}
+
+unsigned *g_arrived = nullptr;  // counters of k_verify, zero between launches
+}  // namespace
+
+void verify_free() {
+    dev_free(g_arrived);
+    g_arrived = nullptr;
+}
+
+namespace {
 // Checks, uploads, runs and waits: *res is the pinned result [n_seq][2 + rows].
 int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, const int32_t *counts, const int32_t *parents,
            const double *u, int n_seq, int rows, int vocab, const int **res) {
     const bool tree = !q;
     if (vocab <= 0 || rows < 1) return set_error(SCRY_ERR_INVALID, "%s: vocabulary and rows must be > 0", what);
+    if (vocab > 1 << 30) return set_error(SCRY_ERR_UNSUPPORTED, "%s: vocabulary %d (at most 2^30)", what, vocab);
     if (rows > VF_MAX_ROWS)
         return set_error(SCRY_ERR_UNSUPPORTED, "%s: %d drafted tokens a sequence (at most %d)", what, rows, VF_MAX_ROWS);
     const int32_t zero[PF_MAX_SEQS] = {};
@@ -235,17 +279,20 @@ int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, cons
     if (!tokens || !u) return set_error(SCRY_ERR_INVALID, "%s: null tokens or random numbers", what);
     const size_t V = vocab, m = rows, n = n_seq * (m + 1);
     if (p->n != n * V || (q && q->n != n_seq * m * V)) return set_error(SCRY_ERR_INVALID, "%s: shape mismatch", what);
-    // workgroups of 256 threads: at least 8 values a thread, at most VF_MAX_CHUNKS chunks
     VfArgs a{};
     a.p = p->d;
     a.q = q ? q->d : nullptr;
     a.V = vocab;
     a.rows = rows;
     a.tree = tree;
-    a.chunk = 2048;
-    while ((V + a.chunk - 1) / a.chunk > VF_MAX_CHUNKS) a.chunk *= 2;
-    a.n_chunk = (int)((V + a.chunk - 1) / a.chunk);
+    a.wide = V % 4 == 0;
     const int R = tree ? rows + 1 : 1;
+    // a wave's part: 512 values (8 a lane), more where that gives more
+    // workgroups than the chip runs at once
+    size_t sub = 512;
+    while (sub < 4096 && (V + 4 * sub - 1) / (4 * sub) * R * n_seq > 2048) sub *= 2;
+    a.sub = (int)sub;
+    a.n_sub = (int)((V + sub - 1) / sub);
 
     VfIn in{};
     double hu[PF_MAX_SEQS * (VF_MAX_ROWS + 1)];
@@ -279,28 +326,30 @@ int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, cons
     std::memcpy(big ? (double *)(host + out_bytes) : in.u, hu, n * sizeof(double));
     std::memcpy(big ? (int *)(host + out_bytes + n * sizeof(double)) : in.tok, ht, n * sizeof(int));
 
-    // workspace: chunk sums, drawn tokens, inputs too many for the arguments
-    const size_t part = (size_t)n_seq * R * 2 * a.n_chunk * sizeof(double), drawn = (n * sizeof(int) + 7) & ~(size_t)7;
+    // workspace: sums of the parts, drawn tokens, inputs too many for the arguments
+    const size_t part = (size_t)n_seq * R * 2 * a.n_sub * sizeof(double), drawn = (n * sizeof(int) + 7) & ~(size_t)7;
     char *ws = nullptr;
     SCRY_TRY(ctx_workspace(part + drawn + n * (sizeof(double) + sizeof(int)), (void **)&ws));
     a.part = (double *)ws;
     a.drawn = (int *)(ws + part);
     hipStream_t st = ctx().stream;
+    if (!g_arrived) {
+        const size_t n_ctr = (size_t)PF_MAX_SEQS * (VF_MAX_ROWS + 2);
+        SCRY_TRY(dev_alloc((void **)&g_arrived, n_ctr * sizeof(unsigned)));
+        const int rc = launch_fill_u32(g_arrived, n_ctr, 0u, st);
+        if (rc) {
+            verify_free();
+            return rc;
+        }
+    }
+    a.arrived = g_arrived;
     if (big) {
         a.u = (double *)(ws + part + drawn);
         a.tok = (int *)(a.u + n);
         SCRY_HIP(hipMemcpyAsync((void *)a.u, host + out_bytes, n * (sizeof(double) + sizeof(int)), hipMemcpyHostToDevice, st));
     }
-    hipLaunchKernelGGL(k_verify_sums, dim3(a.n_chunk, R, n_seq), dim3(256), 0, st, a, in);
+    hipLaunchKernelGGL(k_verify, dim3((a.n_sub + 3) / 4, R, n_seq), dim3(256), 0, st, a, in, d);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess) {
-        hipLaunchKernelGGL(k_verify_draw, dim3(1, R, n_seq), dim3(256), 0, st, a, in);
-        e = hipGetLastError();
-    }
-    if (e == hipSuccess && tree) {
-        hipLaunchKernelGGL(k_verify_walk, dim3(n_seq), dim3(64), 0, st, a, in, d);
-        e = hipGetLastError();
-    }
     // the pinned block is read and written until here, whatever happened
     const hipError_t w = hipStreamSynchronize(st);
     if (e == hipSuccess) e = w;
