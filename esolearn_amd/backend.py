@@ -591,7 +591,7 @@ class HipBackend:
         (paths [n_seq, n], each ended by -1 or by n: as verify_tree returns)."""
         st = _starts(start)
         n_seq = len(st)
-        p = _ints(paths)
+        p = _ints(paths, np.int64)
         if p.ndim != 2 or p.shape[0] != n_seq:
             raise ValueError(f"paths must be [{n_seq}, n]")
         h = _handles(caches, n_seq)

@@ -59,75 +59,203 @@ struct Kv8Rows {
     int rows;
 };
 
-// |x| / s, s > 0, to the nearest integer, halves up, at most 127.  f32 division
-// may round a quotient up to an integer; the remainder x - k s is exact in f32
-// (an fma of a multiple of ulp(s) below 2^24 ulp(s)) and decides.
-__device__ __forceinline__ int steps_of(float x, float s) {
-    const float ax = fabsf(x);
-    const float k = floorf(ax / s);
-    const float e = fmaf(-k, s, ax);
-    const float r = e < 0.f ? k : 2.f * e >= s ? k + 1.f : k;
-    const int q = (int)fminf(r, 127.f);
-    return x < 0.f ? -q : q;
+// Largest value of an aligned group of G lanes, in every lane: quad permutes and
+// mirrors up to 16 lanes, then swaps of rows and halves, none through LDS.
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true)));
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+    v = dpp_max<0xB1>(v);                       // quad_perm [1,0,3,2]
+    v = dpp_max<0x4E>(v);                       // quad_perm [2,3,0,1]
+    if constexpr (G >= 8) v = dpp_max<0x141>(v);   // row_half_mirror
+    if constexpr (G >= 16) v = dpp_max<0x140>(v);  // row_mirror
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return v;
 }
 
-// blockIdx.y: K or V; blockIdx.z: the sequence.  G lanes hold a vector.
+// |x| / s, s > 0, to the nearest integer r, halves up, at most 127.  r is off by
+// one at most before the remainder x - r s, exact in f32 (an fma of a multiple of
+// ulp(s) below 2^24 ulp(s)), decides.
+__device__ __forceinline__ float to_nearest(float ax, float r, float s) {
+    const float e = fmaf(-r, s, ax), e2 = e + e;
+    return fminf(r + (e2 >= s ? 1.f : e2 < -s ? -1.f : 0.f), 127.f);
+}
+
+// A row's four values per lane of a group of G into steps; returns the scale.
+// Rows of ordinary size take the product with 1 / s (to 1 ulp), and look at the
+// remainders once for all four values: 2 |e| >= s is a quotient within rounding
+// of a half, one in 10^5.
+template <int G>
+__device__ __forceinline__ float quantise(float4 x, int (&q)[4]) {
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+    if (__builtin_isunordered(x.x, x.y) || __builtin_isunordered(x.z, x.w)) m = INFINITY;
+    m = group_max<G>(m);
+    if (m >= 0x1p-100f && m < INFINITY) {
+        // m / 127, correctly rounded: the product with f32(1 / 127), its
+        // remainder exact, and one correction
+        const float c = 1.f / 127.f, t = m * c, s = fmaf(fmaf(-127.f, t, m), c, t), inv = __builtin_amdgcn_rcpf(s);
+        float r[4], worst = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            r[i] = rintf(fabsf(v[i]) * inv);
+            worst = fmaxf(worst, fabsf(fmaf(-r[i], s, fabsf(v[i]))));
+        }
+        if (__any(worst + worst >= s)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) r[i] = to_nearest(fabsf(v[i]), r[i], s);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = (int)copysignf(r[i], v[i]);
+        return s;
+    }
+    const float s = m < INFINITY ? m / 127.f : __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        q[i] = s > 0.f ? (int)copysignf(to_nearest(fabsf(v[i]), floorf(fabsf(v[i]) / s), s), v[i]) : 0;
+    return s;
+}
+__device__ __forceinline__ unsigned bytes4(int a, int b, int c, int d) {
+    return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)(d & 255) << 24;
+}
+
+// A workgroup takes one 64-row block of one head, of K or of V (blockIdx.y), of
+// a sequence (blockIdx.z): rows [lo, hi) of the block are the call's.  G lanes
+// hold a row, four dimensions each.
+struct Block {
+    int g, r0, lo, hi;  // head, the block's first cache row, rows of it
+    bool v;
+    size_t src;  // row r of the block is vector src + r * n_kv of the call's rows (lo <= r < hi)
+};
+__device__ __forceinline__ bool block_of(const Kv8Rows &a, Block &b) {
+    const int s = blockIdx.z, start = a.start[s];
+    b.g = blockIdx.x % a.c.n_kv;
+    b.r0 = (start & ~63) + 64 * (int)(blockIdx.x / a.c.n_kv);
+    b.v = blockIdx.y;
+    b.lo = max(start - b.r0, 0);
+    b.hi = min(64, start + a.rows - b.r0);
+    b.src = ((size_t)s * a.rows + (b.r0 - start)) * a.c.n_kv + b.g;  // (wraps below zero where lo > 0: lo takes it back)
+    return b.lo < b.hi;
+}
+constexpr int V_LD = 17;  // words per dimension of a V block in LDS: 16, and one against bank conflicts
+
+// Bound by HBM (4 bytes read, 1 written).  V's 64-byte groups hold one
+// dimension of 64 rows: a whole block is turned through LDS (four rows of a
+// dimension are a word) and written in 16-byte pieces; part of a block in bytes.
+// 2047 rows of 32 heads of 128: 24 us, with V in bytes throughout 54 us.
 template <int G>
 __global__ __launch_bounds__(256) void k_kv8_write(Kv8Rows a, const float *__restrict__ kx, const float *__restrict__ vx) {
     constexpr int NG = 256 / G;
-    const int s = blockIdx.z, tid = threadIdx.x, gl = tid % G;
-    const bool is_v = blockIdx.y;
+    __shared__ unsigned s_v[4 * G * V_LD];
+    Block b;
+    if (!block_of(a, b)) return;
+    const int s = blockIdx.z, tid = threadIdx.x, gl = tid % G, grp = tid / G;
     const int n_kv = a.c.n_kv, hd = a.c.hd, hdp = a.c.hdp, rows_p = a.c.rows_p[s];
-    const size_t n = (size_t)a.rows * n_kv, at = (size_t)blockIdx.x * NG + tid / G;
-    if (at >= n) return;  // whole groups of G lanes leave
-    const int r = a.start[s] + (int)(at / n_kv), g = (int)(at % n_kv);
-    const float *src = (is_v ? vx : kx) + ((size_t)s * n + at) * hd;
     const bool act = 4 * gl < hd;
-    const float4 x = act ? *(const float4 *)(src + 4 * gl) : make_float4(0.f, 0.f, 0.f, 0.f);
-    float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-    if (!(isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w))) m = INFINITY;
+    const float *src = (b.v ? vx : kx) + 4 * gl;
+    float *scales = (b.v ? a.c.vs[s] : a.c.ks[s]) + (size_t)b.g * rows_p + b.r0;
+    auto row = [&](int r) {
+        return act ? *(const float4 *)(src + (b.src + (size_t)r * n_kv) * hd) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    if (b.v && b.lo == 0 && b.hi == 64) {
+        for (int w = grp; w < 16; w += NG) {  // rows 4 w ..
+            float4 x[4];
+            int q[4][4];
 #pragma unroll
-    for (int off = G / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-    const bool bad = m == INFINITY;
-    const float sc = bad ? __builtin_nanf("") : m / 127.f;
-    char4 q = make_char4(0, 0, 0, 0);
-    if (!bad && sc > 0.f)
-        q = make_char4((signed char)steps_of(x.x, sc), (signed char)steps_of(x.y, sc), (signed char)steps_of(x.z, sc),
-                       (signed char)steps_of(x.w, sc));
-    if (is_v) {
-        if (act) {
-            int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, g, r, 4 * gl) + kv8_perm(r & 63);
-            d[0] = q.x ^ 0x80;
-            d[64] = q.y ^ 0x80;
-            d[128] = q.z ^ 0x80;
-            d[192] = q.w ^ 0x80;
+            for (int i = 0; i < 4; i++) x[i] = row(4 * w + i);
+            float sc[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) sc[i] = quantise<G>(x[i], q[i]);
+            if (gl == 0) *(float4 *)(scales + 4 * w) = make_float4(sc[0], sc[1], sc[2], sc[3]);
+            const int at = kv8_perm(4 * w) / 4;
+#pragma unroll
+            for (int e = 0; e < 4; e++) s_v[(4 * gl + e) * V_LD + at] = bytes4(q[0][e], q[1][e], q[2][e], q[3][e]) ^ 0x80808080u;
         }
-    } else if (act) {
-        *(char4 *)(a.c.k[s] + kv8_k_at(rows_p, hdp, g, r) + 4 * gl) = q;
+        __syncthreads();
+        int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 0);
+        for (int t = tid; t < hd * 4; t += 256) {  // dimension t / 4, words 4 (t % 4) ..
+            const unsigned *w = s_v + (t >> 2) * V_LD + 4 * (t & 3);
+            *(uint4 *)(d + 16 * t) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return;
     }
-    if (gl == 0) (is_v ? a.c.vs[s] : a.c.ks[s])[(size_t)g * rows_p + r] = sc;
+#pragma unroll 4
+    for (int r = b.lo + grp; r < b.hi; r += NG) {
+        int q[4];
+        const float sc = quantise<G>(row(r), q);
+        if (gl == 0) scales[r] = sc;
+        if (!act) continue;
+        if (b.v) {
+            int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 4 * gl) + kv8_perm(r);
+#pragma unroll
+            for (int e = 0; e < 4; e++) d[64 * e] = (int8_t)(q[e] ^ 0x80);
+        } else {
+            *(unsigned *)(a.c.k[s] + kv8_k_at(rows_p, hdp, b.g, b.r0 + r) + 4 * gl) = bytes4(q[0], q[1], q[2], q[3]);
+        }
+    }
 }
 
+// The same blocks the other way (1 byte read, 4 written).
 template <int G>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8Rows a, float *__restrict__ kx, float *__restrict__ vx) {
     constexpr int NG = 256 / G;
-    const int s = blockIdx.z, tid = threadIdx.x, gl = tid % G;
-    const bool is_v = blockIdx.y;
+    __shared__ unsigned s_v[4 * G * V_LD];
+    Block b;
+    if (!block_of(a, b)) return;
+    const int s = blockIdx.z, tid = threadIdx.x, gl = tid % G, grp = tid / G;
     const int n_kv = a.c.n_kv, hd = a.c.hd, hdp = a.c.hdp, rows_p = a.c.rows_p[s];
-    const size_t n = (size_t)a.rows * n_kv, at = (size_t)blockIdx.x * NG + tid / G;
-    if (at >= n || 4 * gl >= hd) return;
-    const int r = a.start[s] + (int)(at / n_kv), g = (int)(at % n_kv);
-    const float sc = (is_v ? a.c.vs[s] : a.c.ks[s])[(size_t)g * rows_p + r];
-    char4 q;
-    if (is_v) {
-        const int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, g, r, 4 * gl) + kv8_perm(r & 63);
-        q = make_char4((signed char)(d[0] ^ 0x80), (signed char)(d[64] ^ 0x80), (signed char)(d[128] ^ 0x80),
-                       (signed char)(d[192] ^ 0x80));
-    } else {
-        q = *(const char4 *)(a.c.k[s] + kv8_k_at(rows_p, hdp, g, r) + 4 * gl);
+    const bool act = 4 * gl < hd;
+    float *dst = (b.v ? vx : kx) + 4 * gl;
+    const float *scales = (b.v ? a.c.vs[s] : a.c.ks[s]) + (size_t)b.g * rows_p + b.r0;
+    auto put = [&](int r, unsigned w0, unsigned w1, unsigned w2, unsigned w3, int sh, float sc) {
+        *(float4 *)(dst + (b.src + (size_t)r * n_kv) * hd) =
+            make_float4((float)(int)(signed char)(w0 >> sh) * sc, (float)(int)(signed char)(w1 >> sh) * sc,
+                        (float)(int)(signed char)(w2 >> sh) * sc, (float)(int)(signed char)(w3 >> sh) * sc);
+    };
+    if (b.v && b.lo == 0 && b.hi == 64) {
+        const int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 0);
+        for (int t = tid; t < hd * 4; t += 256) {
+            const uint4 x = *(const uint4 *)(d + 16 * t);
+            unsigned *w = s_v + (t >> 2) * V_LD + 4 * (t & 3);
+            w[0] = x.x ^ 0x80808080u;
+            w[1] = x.y ^ 0x80808080u;
+            w[2] = x.z ^ 0x80808080u;
+            w[3] = x.w ^ 0x80808080u;
+        }
+        __syncthreads();
+        if (!act) return;
+        for (int w = grp; w < 16; w += NG) {
+            const unsigned *x = s_v + 4 * gl * V_LD + kv8_perm(4 * w) / 4;
+            const float4 sc = *(const float4 *)(scales + 4 * w);
+            const unsigned w0 = x[0], w1 = x[V_LD], w2 = x[2 * V_LD], w3 = x[3 * V_LD];
+            put(4 * w, w0, w1, w2, w3, 0, sc.x);
+            put(4 * w + 1, w0, w1, w2, w3, 8, sc.y);
+            put(4 * w + 2, w0, w1, w2, w3, 16, sc.z);
+            put(4 * w + 3, w0, w1, w2, w3, 24, sc.w);
+        }
+        return;
     }
-    *(float4 *)((is_v ? vx : kx) + ((size_t)s * n + at) * hd + 4 * gl) =
-        make_float4((float)q.x * sc, (float)q.y * sc, (float)q.z * sc, (float)q.w * sc);
+    if (!act) return;
+#pragma unroll 4
+    for (int r = b.lo + grp; r < b.hi; r += NG) {
+        const float sc = scales[r];
+        if (b.v) {
+            const uint8_t *d = (const uint8_t *)a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 4 * gl) + kv8_perm(r);
+            put(r, d[0] ^ 0x80u, d[64] ^ 0x80u, d[128] ^ 0x80u, d[192] ^ 0x80u, 0, sc);
+        } else {
+            const unsigned w = *(const unsigned *)(a.c.k[s] + kv8_k_at(rows_p, hdp, b.g, b.r0 + r) + 4 * gl);
+            put(r, w, w >> 8, w >> 16, w >> 24, 0, sc);
+        }
+    }
 }
 
 struct Kv8Keep {
@@ -168,9 +296,9 @@ __global__ __launch_bounds__(256) void k_kv8_keep(Kv8Keep a) {
     if (tid == 0) move(is_v ? a.c.vs[s] : a.c.ks[s], [&](int r) { return (size_t)g * rows_p + r; });
 }
 
-// vectors (row, head) of one sequence per workgroup, by the lanes of a head
+// The lanes that hold a row, as a constant.
 template <class F>
-int by_lanes(int hd, F f) {
+void by_lanes(int hd, F f) {
     const int lanes = hd / 4;
     if (lanes <= 4) return f(std::integral_constant<int, 4>{});
     if (lanes <= 8) return f(std::integral_constant<int, 8>{});
@@ -179,14 +307,22 @@ int by_lanes(int hd, F f) {
     return f(std::integral_constant<int, 64>{});
 }
 
+// Fills a and the grid of the block kernels (one more block than rows / 64 has
+// where a sequence starts inside one).
 int kv8_rows(const char *what, const scry_kv8 *caches, int n_seq, const int32_t *start, int rows, bool distinct,
-             Kv8Rows *a, size_t *n) {
+             Kv8Rows *a, dim3 *grid) {
     DraftBatch d;
     SCRY_TRY(draft_batch(what, n_seq, rows, start, nullptr, &d));
     SCRY_TRY(kv8_batch(what, caches, n_seq, d, rows, distinct, &a->c));
-    for (int s = 0; s < n_seq; s++) a->start[s] = d.len[s];
+    size_t blocks = 0;
+    for (int s = 0; s < n_seq; s++) {
+        a->start[s] = d.len[s];
+        const size_t n = ((size_t)d.len[s] + rows + 63) / 64 - d.len[s] / 64;
+        blocks = blocks > n ? blocks : n;
+    }
     a->rows = rows;
-    *n = (size_t)rows * a->c.n_kv;  // vectors of a sequence
+    if (blocks * a->c.n_kv > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what, rows, a->c.n_kv);
+    *grid = dim3((unsigned)(blocks * a->c.n_kv), 2, n_seq);
     return SCRY_OK;
 }
 
@@ -251,18 +387,16 @@ int scry_hip_kv8_write(const scry_kv8 *caches, int n_seq, const int32_t *start, 
     SCRY_TRY(check_f32(k, "kv8_write"));
     SCRY_TRY(check_f32(v, "kv8_write"));
     Kv8Rows a{};
-    size_t n = 0;
-    SCRY_TRY(kv8_rows("kv8_write", caches, n_seq, start, rows, true, &a, &n));
-    if (k->n != n * n_seq * a.c.hd || v->n != k->n) return set_error(SCRY_ERR_INVALID, "kv8_write: shape mismatch");
+    dim3 grid;
+    SCRY_TRY(kv8_rows("kv8_write", caches, n_seq, start, rows, true, &a, &grid));
+    if (k->n != (size_t)n_seq * rows * a.c.n_kv * a.c.hd || v->n != k->n)
+        return set_error(SCRY_ERR_INVALID, "kv8_write: shape mismatch");
     DeviceScope dev;
-    return by_lanes(a.c.hd, [&](auto g) {
-        constexpr int G = decltype(g)::value, NG = 256 / G;
-        if ((n + NG - 1) / NG > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "kv8_write: %d rows", rows);
-        hipLaunchKernelGGL(k_kv8_write<G>, dim3((unsigned)((n + NG - 1) / NG), 2, n_seq), dim3(256), 0, ctx().stream, a, k->d,
-                           v->d);
-        SCRY_HIP(hipGetLastError());
-        return (int)SCRY_OK;
+    by_lanes(a.c.hd, [&](auto g) {
+        hipLaunchKernelGGL(k_kv8_write<decltype(g)::value>, grid, dim3(256), 0, ctx().stream, a, k->d, v->d);
     });
+    SCRY_HIP(hipGetLastError());
+    return SCRY_OK;
 }
 
 int scry_hip_kv8_read(const scry_kv8 *caches, int n_seq, const int32_t *start, int rows, scry_buf *k, scry_buf *v) {
@@ -270,21 +404,20 @@ int scry_hip_kv8_read(const scry_kv8 *caches, int n_seq, const int32_t *start, i
     SCRY_REQUIRE_INIT();
     if (!k || !v) return set_error(SCRY_ERR_INVALID, "kv8_read: null output handle");
     Kv8Rows a{};
-    size_t n = 0;
-    SCRY_TRY(kv8_rows("kv8_read", caches, n_seq, start, rows, false, &a, &n));
+    dim3 grid;
+    SCRY_TRY(kv8_rows("kv8_read", caches, n_seq, start, rows, false, &a, &grid));
+    const size_t n = (size_t)n_seq * rows * a.c.n_kv * a.c.hd;
     DeviceScope dev;
     scry_buf ok = nullptr, ov = nullptr;
-    int rc = buf_new(n * n_seq * a.c.hd, &ok);
-    if (!rc) rc = buf_new(n * n_seq * a.c.hd, &ov);
-    if (!rc)
-        rc = by_lanes(a.c.hd, [&](auto g) {
-            constexpr int G = decltype(g)::value, NG = 256 / G;
-            if ((n + NG - 1) / NG > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "kv8_read: %d rows", rows);
-            hipLaunchKernelGGL(k_kv8_read<G>, dim3((unsigned)((n + NG - 1) / NG), 2, n_seq), dim3(256), 0, ctx().stream, a,
-                               ok->d, ov->d);
-            SCRY_HIP(hipGetLastError());
-            return (int)SCRY_OK;
+    int rc = buf_new(n, &ok);
+    if (!rc) rc = buf_new(n, &ov);
+    if (!rc) {
+        by_lanes(a.c.hd, [&](auto g) {
+            hipLaunchKernelGGL(k_kv8_read<decltype(g)::value>, grid, dim3(256), 0, ctx().stream, a, ok->d, ov->d);
         });
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) rc = hip_fail(e, "kv8_read", __FILE__, __LINE__);
+    }
     if (rc) {
         buf_del(ok);
         buf_del(ov);
@@ -295,7 +428,7 @@ int scry_hip_kv8_read(const scry_kv8 *caches, int n_seq, const int32_t *start, i
     return SCRY_OK;
 }
 
-int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, const int32_t *paths, int n_path) {
+int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, const int64_t *paths, int n_path) {
     API_LOCK;
     SCRY_REQUIRE_INIT();
     const char *what = "kv8_keep";
@@ -306,12 +439,12 @@ int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, c
     Kv8Keep a{};
     bool moves = false;
     for (int s = 0; s < n_seq; s++) {
-        const int32_t *p = paths + (size_t)s * n_path;
+        const int64_t *p = paths + (size_t)s * n_path;
         int n = 0;
         while (n < n_path && p[n] != -1) {
             if (p[n] < 0 || p[n] >= DRAFT_MAX_TREE || (n && p[n] <= p[n - 1]))
-                return set_error(SCRY_ERR_INVALID, "%s: node %d at place %d of sequence %d's path (ascending, below %d)", what,
-                                 p[n], n, s, DRAFT_MAX_TREE);
+                return set_error(SCRY_ERR_INVALID, "%s: node %lld at place %d of sequence %d's path (ascending, below %d)", what,
+                                 (long long)p[n], n, s, DRAFT_MAX_TREE);
             a.path[s][n] = (unsigned char)p[n];
             moves |= p[n] != n;
             n++;
@@ -319,7 +452,7 @@ int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, c
         a.count[s] = n;
         a.start[s] = d.len[s];
         if (n && caches && caches[s] && (long long)d.len[s] + p[n - 1] >= caches[s]->max_seq)
-            return set_error(SCRY_ERR_RANGE, "%s: row %d + %d of cache %d, which holds %d", what, d.len[s], p[n - 1], s,
+            return set_error(SCRY_ERR_RANGE, "%s: row %d + %d of cache %d, which holds %d", what, d.len[s], (int)p[n - 1], s,
                              caches[s]->max_seq);
     }
     SCRY_TRY(kv8_batch(what, caches, n_seq, d, 0, true, &a.c));

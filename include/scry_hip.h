@@ -292,9 +292,10 @@ int scry_hip_kv8_write(const scry_kv8 *caches, int n_seq, const int32_t *start, 
  * head_dim].  Rows never written are zero. */
 int scry_hip_kv8_read(const scry_kv8 *caches, int n_seq, const int32_t *start, int rows, scry_buf *k, scry_buf *v);
 /* The accepted path's rows move up: row start + paths[s][i] to start + i, for
- * every i below n_path (at most 64) or the first -1.  A path is ascending
- * nodes below 64; it may be empty. */
-int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, const int32_t *paths, int n_path);
+ * every i below n_path (at most 64) or the first -1 (paths [n_seq][n_path], as
+ * verify_tree gives them).  A path is ascending nodes below 64; it may be
+ * empty. */
+int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, const int64_t *paths, int n_path);
 
 /* Attention of the drafted rows: q [n_seq * rows, n_q * head_dim]; row i of a
  * sequence attends to its cache rows [0, len) and to len + j of its ancestors j

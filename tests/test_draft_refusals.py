@@ -190,8 +190,9 @@ st("kv8_write", h1, 1, one, rows, k.h, None)
 st("kv8_read", h1, 1, one, rows, r(C.c_void_p()), None)
 st("kv8_read", None, 1, one, rows, r(C.c_void_p()), r(C.c_void_p()))
 st("kv8_keep", h1, 1, one, None, 1)
-st("kv8_keep", None, 1, one, one, 1)
-st("kv8_keep", n1, 1, one, one, 1)
+long = (C.c_int64 * 1)(1)
+st("kv8_keep", None, 1, one, long, 1)
+st("kv8_keep", n1, 1, one, long, 1)
 st("tree_attention", q.h, None, n1, 1, one, rows, None, nq, nkv, hd, 0.1, r(C.c_void_p()))
 st("tree_attention", q.h, n1, n1, 1, one, rows, None, nq, nkv, hd, 0.1, r(C.c_void_p()))
 st("tree_attention", q.h, (C.c_void_p * 1)(kc.h), (C.c_void_p * 1)(vc.h), 1, one, rows, None, nq, nkv, hd, 0.1, None)
