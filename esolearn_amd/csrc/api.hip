@@ -417,8 +417,7 @@ int scry_hip_shutdown(void) {
     Ctx &c = ctx();
     if (!c.init) return SCRY_OK;
     (void)hipStreamSynchronize(c.stream);
-    host_block_free();
-    verify_free();
+    draft_free();
     pool_trim();
     dev_free(c.ws);
     (void)hipStreamDestroy(c.stream);

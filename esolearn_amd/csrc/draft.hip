@@ -52,12 +52,19 @@ int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, con
 namespace {
 void *g_host = nullptr;
 size_t g_host_bytes = 0;
+unsigned *g_counters = nullptr;
+
+void host_free() {
+    if (g_host) (void)hipHostFree(g_host);
+    g_host = nullptr;
+    g_host_bytes = 0;
+}
 }  // namespace
 
 int host_block(size_t bytes, void **p) {
     if (g_host_bytes < bytes) {
         SCRY_HIP(hipStreamSynchronize(ctx().stream));
-        host_block_free();
+        host_free();
         const size_t want = (bytes + 4095) & ~(size_t)4095;
         SCRY_HIP(hipHostMalloc(&g_host, want, hipHostMallocDefault));
         g_host_bytes = want;
@@ -66,10 +73,25 @@ int host_block(size_t bytes, void **p) {
     return SCRY_OK;
 }
 
-void host_block_free() {
-    if (g_host) (void)hipHostFree(g_host);
-    g_host = nullptr;
-    g_host_bytes = 0;
+int draft_counters(unsigned **ctr) {
+    if (!g_counters) {
+        void *p = nullptr;
+        SCRY_TRY(dev_alloc(&p, DRAFT_COUNTERS * sizeof(unsigned)));
+        const int rc = launch_fill_u32((unsigned *)p, DRAFT_COUNTERS, 0u, ctx().stream);
+        if (rc) {
+            dev_free(p);
+            return rc;
+        }
+        g_counters = (unsigned *)p;
+    }
+    *ctr = g_counters;
+    return SCRY_OK;
+}
+
+void draft_free() {
+    host_free();
+    dev_free(g_counters);
+    g_counters = nullptr;
 }
 
 namespace {

@@ -468,8 +468,10 @@ int check_heads(const char *what, int n_q, int n_kv, int head_dim);  // n_q = 0:
 // pinned host memory that the device reads and writes, `bytes` large, kept until shutdown; its users wait
 // for the stream before they return
 int host_block(size_t bytes, void **p);
-void host_block_free();
-void verify_free();  // verify.hip: its counters
+// arrival counters (arrive.h) of the launches on the context's stream, zero between them
+constexpr size_t DRAFT_COUNTERS = 16384;
+int draft_counters(unsigned **ctr);
+void draft_free();  // the pinned block and the counters, at shutdown
 
 // bf16.hip -- bf16 mode: the reference's cast, widening, B-operand rows
 // [n][kp] (kp = bf16_row_pad(k)), the GEMM activation plane, the bf16 GEMV

@@ -19,6 +19,7 @@
 // after the first.
 #include <cmath>
 
+#include "arrive.h"
 #include "kdev.h"
 #include "kv8.h"
 
@@ -47,6 +48,7 @@ struct TreeArgs {
     int n_split, n_qg;  // n_qg: groups of the workgroup's columns
     int splits[PF_MAX_SEQS], pair0[PF_MAX_SEQS + 1];
     float scale2;                   // scale * log2(e)
+    unsigned *arrived;  // splits per (sequence, KV head, column group), zero between launches; null: k_tree_merge* join
 };
 
 constexpr int WAVES = 4;
@@ -140,6 +142,54 @@ __device__ __forceinline__ void store_out(const TreeArgs &a, int s, int g, int c
 __device__ __forceinline__ size_t part_of(const TreeArgs &a, const Unit &u, int c) {
     return (((size_t)u.s * a.n_kv + u.g) * a.cols + c) * a.n_split + u.split;
 }
+// A split's partial: read in this launch by the last split to arrive (put /
+// get), or by the next launch.
+__device__ __forceinline__ void store_part(const TreeArgs &a, size_t at, int d, float4 v) {
+    float *p = a.part_o + at * a.hd + d;
+    if (a.arrived) {
+        put((unsigned long long *)p, __builtin_bit_cast(unsigned long long, make_float2(v.x, v.y)));
+        put((unsigned long long *)p + 1, __builtin_bit_cast(unsigned long long, make_float2(v.z, v.w)));
+    } else {
+        *(float4 *)p = v;
+    }
+}
+__device__ __forceinline__ void store_ml(const TreeArgs &a, size_t at, float c, float l) {
+    float *p = a.part_ml + at * 2;
+    if (a.arrived)
+        put((unsigned long long *)p, __builtin_bit_cast(unsigned long long, make_float2(c, l)));
+    else
+        *(float2 *)p = make_float2(c, l);
+}
+__device__ __forceinline__ float2 get2(const float *p) {
+    return __builtin_bit_cast(float2, get((const unsigned long long *)p));
+}
+__device__ __forceinline__ bool last_split(const TreeArgs &a, const Unit &u) {
+    return last_to_arrive(a.arrived + ((size_t)u.s * a.n_kv + u.g) * a.n_qg + u.qg, a.splits[u.s]);
+}
+
+// The tile of a wide kernel's wave: a wave stays on its SIMD, so tiles that are
+// not there (seven in two groups of four) go round.
+template <int W>
+__device__ __forceinline__ int tile_of(const Unit &u, int wave) {
+    return (wave + u.g + u.split) % W;
+}
+
+// A wide kernel's wave ends: the output of its columns, or a split's partial.
+template <int N, class DIM>
+__device__ __forceinline__ void finish_wide(const TreeArgs &a, const Unit &u, int c, float own_c, float own_l, float4 (&o)[N], DIM dim) {
+    if (c >= a.cols) return;
+    const size_t at = part_of(a, u, c);
+    const float inv = 1.f / own_l;
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        if (dim(x) >= a.hd) continue;
+        if (a.n_split == 1)
+            store_out(a, u.s, u.g, c, dim(x), o[x], inv);
+        else
+            *(float4 *)(a.part_o + at * a.hd + dim(x)) = o[x];
+    }
+    if (a.n_split > 1 && (threadIdx.x & 63) < 16) *(float2 *)(a.part_ml + at * 2) = make_float2(own_c, own_l);
+}
 
 // The four waves' (c, sum, out) of each column joined in wave order, from
 // s_o [wave][column][ld], s_c and s_l [wave][column]: the output, or one split's
@@ -172,9 +222,47 @@ __device__ __forceinline__ void join_waves(const TreeArgs &a, const Unit &u, con
             store_out(a, u.s, u.g, c, d, o, 1.f / L);
         } else {
             const size_t at = part_of(a, u, c);
-            *(float4 *)(a.part_o + at * hd + d) = o;
-            if (d == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(C, L);
+            store_part(a, at, d, o);
+            if (d == 0) store_ml(a, at, C, L);
         }
+    }
+    if (a.n_split == 1 || !a.arrived || !last_split(a, u)) return;
+    // the last split of these columns: a thread per four dimensions
+    const int ns = a.splits[u.s];
+    for (int x = threadIdx.x; x < COLS * n4; x += 64 * WAVES) {
+        const int d = 4 * (x % n4), c = u.qg * COLS + x / n4;
+        if (c >= a.cols) break;
+        const size_t at = part_of(a, u, c) - u.split;
+        float C = -INFINITY, L = 0.f;
+        float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = 0; p0 < ns; p0 += 8) {  // eight splits' loads before their first use
+            float2 ml[8], lo[8], hi[8];
+#pragma unroll
+            for (int p = 0; p < 8; p++) {
+                const size_t q = at + min(p0 + p, ns - 1);
+                ml[p] = get2(a.part_ml + q * 2);
+                lo[p] = get2(a.part_o + q * hd + d);
+                hi[p] = get2(a.part_o + q * hd + d + 2);
+            }
+            float top = C;
+#pragma unroll
+            for (int p = 0; p < 8; p++) top = fmaxf(top, ml[p].x);
+            const float ref = top == -INFINITY ? 0.f : top, f0 = exp2_fast(C - ref);
+            C = top;
+            L *= f0;
+            r = make_float4(r.x * f0, r.y * f0, r.z * f0, r.w * f0);
+#pragma unroll
+            for (int p = 0; p < 8; p++) {
+                if (p0 + p >= ns) break;
+                const float f = exp2_fast(ml[p].x - ref);
+                L += ml[p].y * f;
+                r.x += lo[p].x * f;
+                r.y += lo[p].y * f;
+                r.z += hi[p].x * f;
+                r.w += hi[p].y * f;
+            }
+        }
+        store_out(a, u.s, u.g, c, d, r, 1.f / L);
     }
 }
 
@@ -394,7 +482,7 @@ __device__ __forceinline__ void split_weights(const float (&w)[4], int x, f16x8 
 // of w.v.  Where the reference moves, l is rescaled and o's factor is returned
 // (1: o stays).  The reference need not be the largest score: it is kept while
 // the weights fit f16 and the sum f32, so most steps neither look for a
-// maximum nor rescale (64-node trees of eight 4000-row contexts: VARIANT).
+// maximum nor rescale (a 512-row chunk over 1500 rows of 32 heads: 63 -> 58 us).
 template <class KQ, class VS>
 __device__ __forceinline__ float softmax_step(RunI8 &r, const f32x4 (&sc)[4], KQ &&kq, VS &&vs, bool full, const Column &co, int t,
                                               int len, f16x8 (&wh)[2], f16x8 (&wl)[2]) {
@@ -570,7 +658,7 @@ __global__ __launch_bounds__(64 * W, (KS == 1 ? 4 : KS == 2 ? 3 : 2) - (W < 4 ? 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cl = lane & 15, j = lane >> 4;
     const int hd = a.hd, hdp = cb.hdp, len = a.d.len[u.s];
-    const int c0 = (u.qg * W + wave) * 16, c = c0 + cl;
+    const int c0 = (u.qg * W + tile_of<W>(u, wave)) * 16, c = c0 + cl;
     const Column co = column_of(a, u.s, c, a.d.tree ? ancestor_mask(a.d, u.s) : 0);
     i32x4 qd[3][KS];
     const float qs = query_digits<KS>(a, u, c, j, qd);
@@ -652,20 +740,10 @@ __global__ __launch_bounds__(64 * W, (KS == 1 ? 4 : KS == 2 ? 3 : 2) - (W < 4 ? 
             }
     }
 
-    const float sum = col_sum(r.l);
-    if (c >= a.cols) return;
-    const size_t at = part_of(a, u, c);
+    float4 v[DT];
 #pragma unroll
-    for (int d = 0; d < DT; d++) {
-        const int dd = 16 * d + 4 * j;
-        if (dd >= hd) break;
-        const float4 v = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-        if (a.n_split == 1)
-            store_out(a, u.s, u.g, c, dd, v, 1.f / sum);
-        else
-            *(float4 *)(a.part_o + at * hd + dd) = v;
-    }
-    if (a.n_split > 1 && j == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(r.c, sum);
+    for (int d = 0; d < DT; d++) v[d] = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+    finish_wide(a, u, c, r.c, col_sum(r.l), v, [&](int d) { return 16 * d + 4 * j; });
 }
 
 // ------------------------------------------------------------- f32 cache
@@ -862,7 +940,7 @@ __global__ __launch_bounds__(64 * W, ET <= 2 ? 3 : ET == 4 && W == 2 ? 1 : 2) vo
     const int cl = lane & 15, j = lane >> 4;
     const int hd = a.hd, len = a.d.len[u.s], ldk = a.n_kv * hd, rows_end = len + a.d.rows;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    const int c0 = (u.qg * W + wave) * 16, c = c0 + cl;
+    const int c0 = (u.qg * W + tile_of<W>(u, wave)) * 16, c = c0 + cl;
     const Column co = column_of(a, u.s, c, a.d.tree ? ancestor_mask(a.d, u.s) : 0);
     const int end = c0 >= a.cols ? 0 : a.d.tree ? rows_end : len + min(c0 + 15, a.cols - 1) / a.nrep + 1;
     f32x4 q[CT], o[ET][4];
@@ -967,22 +1045,12 @@ __global__ __launch_bounds__(64 * W, ET <= 2 ? 3 : ET == 4 && W == 2 ? 1 : 2) vo
         }
     }
 
-    const float sum = col_sum(l), inv = 1.f / sum;
-    if (c >= a.cols) return;
-    const size_t at = part_of(a, u, c);
+    float4 v[4 * ET];
 #pragma unroll
     for (int e = 0; e < ET; e++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int d = 64 * e + 16 * j + 4 * r;
-            if (d >= hd) continue;
-            const float4 v = make_float4(o[e][0][r], o[e][1][r], o[e][2][r], o[e][3][r]);
-            if (a.n_split == 1)
-                store_out(a, u.s, u.g, c, d, v, inv);
-            else
-                *(float4 *)(a.part_o + at * hd + d) = v;
-        }
-    if (a.n_split > 1 && j == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(m, sum);
+        for (int r = 0; r < 4; r++) v[4 * e + r] = make_float4(o[e][0][r], o[e][1][r], o[e][2][r], o[e][3][r]);
+    finish_wide(a, u, c, m, col_sum(l), v, [&](int x) { return 64 * (x / 4) + 16 * j + 4 * (x % 4); });
 }
 
 // Key splits: about `want` workgroups in all, each of `least` steps or more,
@@ -1003,7 +1071,7 @@ void pick_splits(TreeArgs &a, int step_keys, int want, int least) {
 
 // waves: of a workgroup; cols: its columns
 template <class K, class B>
-int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t lds, int step_keys, int want, int least, hipStream_t s) {
+int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t lds, int step_keys, int want, int least, int fused, hipStream_t s) {
     a.n_qg = (a.cols + cols - 1) / cols;
     pick_splits(a, step_keys, want, least);
     const size_t n_col = (size_t)a.d.n_seq * a.n_kv * a.cols;
@@ -1017,18 +1085,26 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
     }
     const size_t grid = (size_t)((a.pair0[a.d.n_seq] + 7) / 8) * 8 * a.n_qg;
     if (grid > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "attention: %zu workgroups", grid);
+    // Few splits of few columns: the last to arrive joins them, without a second
+    // launch (one token, 4 query heads a KV head, over 2000 rows: 15.9 -> 12.7
+    // us).  The wide kernels' columns are joined by a launch of their own, which
+    // has more workgroups for it (trees of eight 4000-row contexts: 79 us against
+    // 88 us joined by the last).
+    a.arrived = nullptr;
+    if (a.n_split > 1 && a.n_split <= fused && (size_t)a.d.n_seq * a.n_kv * a.n_qg <= DRAFT_COUNTERS) SCRY_TRY(draft_counters(&a.arrived));
     if (lds > 65536)
         SCRY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), lds, s, a, b);
     SCRY_HIP(hipGetLastError());
     // a thread per four dimensions where they fill the chip, else the groups of
-    // k_tree_merge (16384 columns of 128 by 3 splits: 8 against 13 us; 32 by 64:
-    // 4 against MERGEFLAT us)
+    // k_tree_merge (16384 columns of 128 by 3 splits: 8 against 13 us; 32 columns
+    // by 64 splits: 19 against 4 us)
     const size_t n = n_col * (a.hd / 4);
-    if (a.n_split > 1 && n >= (size_t)1 << 15) {
+    if (a.n_split == 1 || a.arrived) return SCRY_OK;
+    if (n >= (size_t)1 << 15) {
         hipLaunchKernelGGL(k_tree_merge_flat, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, n);
         SCRY_HIP(hipGetLastError());
-    } else if (a.n_split > 1) {
+    } else {
         int lanes = 1;
         while (4 * lanes < a.hd) lanes *= 2;
         // threads of a column: its lanes, times up to as many groups as it has splits
@@ -1041,33 +1117,33 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
     return SCRY_OK;
 }
 
-#ifndef WANT1
-#define WANT1 768
-#define LEAST1 8
-#define WANTW 768
-#define LEASTW 4
-#define WANTF 768
-#define LEASTF 8
-#define WANTFW 768
-#define LEASTFW 4
-#endif
+// Workgroups that a launch aims at: three of four waves a CU (what the wide
+// int8 kernel's registers allow at 128 dimensions: 64-node trees of eight
+// 4000-row contexts 97 us at two, 79 at three, 97 at four, of which some wait).
+// The f32 kernels: 26-node trees of four 2047-row contexts 57.7 us at two, 56.1
+// at three, 66.9 at four.
+constexpr int WANT = 768;
+constexpr int FUSED = 16;  // key splits that the last of a narrow kernel's workgroups joins
+
+// Columns in tiles of 16: three or four tiles share the keys (W waves).  One tile,
+// over int8 caches two, have the narrow kernel (8-node trees of 32 columns over
+// 2000 rows of four sequences: int8 23.4 us wide, 17.6 narrow, f32 35.2 and 39.7).
 template <int KS>
 int launch_i8(const TreeArgs &a, const Kv8Batch &b, hipStream_t s) {
     const int tiles = (a.cols + 15) / 16, groups = (tiles + 3) / 4, w = (tiles + groups - 1) / groups;
     const size_t lds = (size_t)WAVES * 16 * (a.hd + 4 + 2) * sizeof(float);
-    if (w == 1) return launch_tree(k_tree_i8<KS>, a, b, WAVES, 16, lds, 64, WANT1, LEAST1, s);
-    if (w == 2) return launch_tree(k_tree_i8_wide<KS, 2>, a, b, 2, 32, 0, 64, 2 * WANTW, LEASTW, s);
-    if (w == 3) return launch_tree(k_tree_i8_wide<KS, 3>, a, b, 3, 48, 0, 64, 4 * WANTW / 3, LEASTW, s);
-    return launch_tree(k_tree_i8_wide<KS, 4>, a, b, 4, 64, 0, 64, WANTW, LEASTW, s);
+    if (tiles <= 2) return launch_tree(k_tree_i8<KS>, a, b, WAVES, 16, lds, 64, WANT, 8, FUSED, s);
+    if (w == 3) return launch_tree(k_tree_i8_wide<KS, 3>, a, b, 3, 48, 0, 64, 4 * WANT / 3, 4, 0, s);
+    return launch_tree(k_tree_i8_wide<KS, 4>, a, b, 4, 64, 0, 64, WANT, 4, 0, s);
 }
 template <int ET>
 int launch_f32(const TreeArgs &a, const F32Batch &b, hipStream_t s) {
     const int tiles = (a.cols + 15) / 16, groups = (tiles + 3) / 4, w = (tiles + groups - 1) / groups;
     const size_t lds = (size_t)WAVES * 16 * (a.hd + 4 + 2) * sizeof(float);
-    if (w == 1) return launch_tree(k_tree_f32<ET>, a, b, WAVES, 16, lds, 16, WANTF, LEASTF, s);
-    if (w == 2) return launch_tree(k_tree_f32_wide<ET, 2>, a, b, 2, 32, 0, 16 * tree_f32_blocks(ET), 2 * WANTFW, LEASTFW, s);
-    if (w == 3) return launch_tree(k_tree_f32_wide<ET, 3>, a, b, 3, 48, 0, 16 * tree_f32_blocks(ET), 4 * WANTFW / 3, LEASTFW, s);
-    return launch_tree(k_tree_f32_wide<ET, 4>, a, b, 4, 64, 0, 16 * tree_f32_blocks(ET), WANTFW, LEASTFW, s);
+    if (w == 1) return launch_tree(k_tree_f32<ET>, a, b, WAVES, 16, lds, 16, WANT, 8, FUSED, s);
+    if (w == 2) return launch_tree(k_tree_f32_wide<ET, 2>, a, b, 2, 32, 0, 16 * tree_f32_blocks(ET), 2 * WANT, 4, 0, s);
+    if (w == 3) return launch_tree(k_tree_f32_wide<ET, 3>, a, b, 3, 48, 0, 16 * tree_f32_blocks(ET), 4 * WANT / 3, 4, 0, s);
+    return launch_tree(k_tree_f32_wide<ET, 4>, a, b, 4, 64, 0, 16 * tree_f32_blocks(ET), WANT, 4, 0, s);
 }
 
 int tree_run(const char *what, scry_buf q, const TreeArgs &t, bool i8, const F32Batch &f, const Kv8Batch &c, scry_buf *out) {

@@ -23,6 +23,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "arrive.h"
 #include "internal.h"
 #include "kdev.h"
 
@@ -57,33 +58,6 @@ __device__ __forceinline__ double weight(float p) { return p > 0.f && p < INFINI
 __device__ __forceinline__ double weight(float p, float q) {
     const double w = (double)p - (double)q;
     return w > 0.0 && w < (double)INFINITY ? w : 0.0;
-}
-
-// Values that other workgroups, on other XCDs, read in this launch: device-scope
-// accesses go past the XCD's own L2.
-template <class T>
-__device__ __forceinline__ void put(T *p, T v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-template <class T>
-__device__ __forceinline__ T get(const T *p) {
-    return __hip_atomic_load(const_cast<T *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-// With every thread of the workgroup: whether it is the last of n to arrive.
-// What the others put before they arrived, it gets: each wave waits until its
-// device-scope stores are complete, then the barrier, then the count.  (A
-// release fence would write back the XCD's whole L2, once a workgroup: 16
-// sequences at V = 128256 took 91 us with it.)
-__device__ __forceinline__ bool last_to_arrive(unsigned *ctr, unsigned n) {
-    __shared__ int s_last;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s_last = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
-        if (s_last) put(ctr, 0u);  // for the next launch
-    }
-    __syncthreads();
-    return s_last;
 }
 
 // What sequence s draws from: row p, less row q where it is set.  For a chain
@@ -256,15 +230,6 @@ __global__ __launch_bounds__(256) void k_verify(VfArgs a, VfIn in, DraftBatch d)
     if (wave == 0) vf_walk(a, in, d, s);
 }
 
-unsigned *g_arrived = nullptr;  // counters of k_verify, zero between launches
-}  // namespace
-
-void verify_free() {
-    dev_free(g_arrived);
-    g_arrived = nullptr;
-}
-
-namespace {
 // Checks, uploads, runs and waits: *res is the pinned result [n_seq][2 + rows].
 int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, const int32_t *counts, const int32_t *parents,
            const double *u, int n_seq, int rows, int vocab, const int **res) {
@@ -333,16 +298,8 @@ int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, cons
     a.part = (double *)ws;
     a.drawn = (int *)(ws + part);
     hipStream_t st = ctx().stream;
-    if (!g_arrived) {
-        const size_t n_ctr = (size_t)PF_MAX_SEQS * (VF_MAX_ROWS + 2);
-        SCRY_TRY(dev_alloc((void **)&g_arrived, n_ctr * sizeof(unsigned)));
-        const int rc = launch_fill_u32(g_arrived, n_ctr, 0u, st);
-        if (rc) {
-            verify_free();
-            return rc;
-        }
-    }
-    a.arrived = g_arrived;
+    static_assert((size_t)PF_MAX_SEQS * (VF_MAX_ROWS + 2) <= DRAFT_COUNTERS, "counters");
+    SCRY_TRY(draft_counters(&a.arrived));
     if (big) {
         a.u = (double *)(ws + part + drawn);
         a.tok = (int *)(a.u + n);
