@@ -18,21 +18,7 @@ from ._lib import call, load
 
 _CAPSULE_NEW = C.pythonapi.PyCapsule_New
 _CAPSULE_NEW.restype, _CAPSULE_NEW.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
-C.pythonapi.PyCapsule_IsValid.argtypes = [C.c_void_p, C.c_char_p]
-C.pythonapi.PyCapsule_GetPointer.restype = C.c_void_p
-C.pythonapi.PyCapsule_GetPointer.argtypes = [C.c_void_p, C.c_char_p]
-
-
-@C.PYFUNCTYPE(None, C.c_void_p)
-def _capsule_end(capsule):
-    """A capsule that nobody took (who takes one renames it) ends its view."""
-    if C.pythonapi.PyCapsule_IsValid(capsule, b"dltensor"):
-        m = C.pythonapi.PyCapsule_GetPointer(capsule, b"dltensor")
-        deleter = C.cast(m + 56, C.POINTER(C.CFUNCTYPE(None, C.c_void_p)))[0]  # after the tensor (48 bytes) and the context
-        deleter(m)
-
-
-_CAPSULE_END = C.cast(_capsule_end, C.c_void_p)
+_capsule_end = None  # the library's destructor of such capsules, on first use
 
 
 def _f32(a) -> np.ndarray:
@@ -63,9 +49,12 @@ class Storage:
         the ops called so far (None, 0, 1: the default stream); -1: the caller
         waits, as with HipBackend.synchronize().  Writes through the view, and
         reads that outlive it, are ordered by the caller."""
+        global _capsule_end
+        if _capsule_end is None:
+            _capsule_end = C.cast(load().scry_hip_dlpack_capsule_end, C.c_void_p)
         m = C.c_void_p()
-        call("scry_hip_buf_dlpack", self.h, None if stream in (None, 0, 1, -1) else stream, int(stream != -1), C.byref(m))
-        return _CAPSULE_NEW(m, b"dltensor", _CAPSULE_END)
+        call("scry_hip_buf_dlpack", self.h, None if stream in (None, 0, 1, -1) else stream, stream != -1, C.byref(m))
+        return _CAPSULE_NEW(m, b"dltensor", _capsule_end)
 
     def free(self) -> None:
         if self.h:
@@ -162,7 +151,7 @@ def _parents(parents, n_seq: int, rows: int):
     """[n_seq, rows] parents, or one tree [rows] that every sequence has."""
     if parents is None:
         return None, None
-    a = _ints(parents)
+    a = _ints(parents, np.int64)
     if a.shape == (rows,):
         a = np.ascontiguousarray(np.broadcast_to(a, (n_seq, rows)))
     if a.shape != (n_seq, rows):

@@ -8,6 +8,8 @@
 #include <cstring>
 #include <vector>
 
+#include <dlfcn.h>
+
 #include "internal.h"
 
 namespace scry {
@@ -612,6 +614,15 @@ int scry_hip_buf_dlpack(scry_buf b, void *wait_stream, int wait, void **managed)
     };
     *managed = v;
     return SCRY_OK;
+}
+
+void scry_hip_dlpack_capsule_end(void *capsule) {
+    // the interpreter's functions, of the process that calls this (the library does not link Python)
+    static const auto valid = (int (*)(void *, const char *))dlsym(RTLD_DEFAULT, "PyCapsule_IsValid");
+    static const auto pointer = (void *(*)(void *, const char *))dlsym(RTLD_DEFAULT, "PyCapsule_GetPointer");
+    if (!valid || !pointer || !valid(capsule, "dltensor")) return;
+    auto *v = (DlView *)pointer(capsule, "dltensor");
+    if (v) v->deleter(v);
 }
 
 int scry_hip_free(scry_buf b) {

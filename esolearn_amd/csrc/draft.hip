@@ -24,7 +24,7 @@ int check_heads(const char *what, int n_q, int n_kv, int head_dim) {
     return SCRY_OK;
 }
 
-int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, const int32_t *parents, DraftBatch *b) {
+int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, const int64_t *parents, DraftBatch *b) {
     if (n_seq < 1 || n_seq > PF_MAX_SEQS)
         return set_error(SCRY_ERR_INVALID, "%s: %d sequences (1..%d)", what, n_seq, PF_MAX_SEQS);
     if (rows < 1 || !start) return set_error(SCRY_ERR_INVALID, "%s: rows and start", what);
@@ -39,10 +39,10 @@ int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, con
             return set_error(SCRY_ERR_RANGE, "%s: sequence %d starts at row %d", what, s, start[s]);
         b->len[s] = start[s];
         for (int i = 0; parents && i < rows; i++) {
-            const int p = parents[(size_t)s * rows + i];
+            const int64_t p = parents[(size_t)s * rows + i];
             if (p < -2 || p >= i || (p >= 0 && b->parent[s][p] == -2))
-                return set_error(SCRY_ERR_INVALID, "%s: node %d of sequence %d has parent %d (an earlier node, -1: the context, -2: no node)",
-                                 what, i, s, p);
+                return set_error(SCRY_ERR_INVALID, "%s: node %d of sequence %d has parent %lld (an earlier node, -1: the context, -2: no node)",
+                                 what, i, s, (long long)p);
             b->parent[s][i] = (signed char)p;
         }
     }
@@ -174,7 +174,7 @@ int launch_qk(const QkArgs &a, int n_rows, hipStream_t s) {
 
 using namespace scry;
 
-extern "C" int scry_hip_qk_norm_rope(scry_buf qkv, int n_seq, int rows, const int32_t *start, const int32_t *parents,
+extern "C" int scry_hip_qk_norm_rope(scry_buf qkv, int n_seq, int rows, const int32_t *start, const int64_t *parents,
                                      int n_q, int n_kv, int head_dim, scry_buf freqs, scry_buf q_weight,
                                      scry_buf k_weight, float eps, float q_scale, scry_buf *q, scry_buf *k, scry_buf *v) {
     std::lock_guard<std::recursive_mutex> lock(api_mutex());

@@ -463,7 +463,7 @@ struct DraftBatch {                 // passed to kernels by value
     signed char parent[PF_MAX_SEQS][DRAFT_MAX_TREE];  // tree: -1 the context, -2 no node
 };
 // Checks start and parents (host, [n_seq] and [n_seq][rows] or null) and fills b.
-int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, const int32_t *parents, DraftBatch *b);
+int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, const int64_t *parents, DraftBatch *b);
 int check_heads(const char *what, int n_q, int n_kv, int head_dim);  // n_q = 0: no query heads
 // pinned host memory that the device reads and writes, `bytes` large, kept until shutdown; its users wait
 // for the stream before they return

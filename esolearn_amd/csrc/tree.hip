@@ -271,15 +271,15 @@ __device__ __forceinline__ void join_waves(const TreeArgs &a, const Unit &u, con
 // threads sum its splits, lanes of four dimensions times groups of splits, and
 // the groups are joined through LDS.
 constexpr int MAX_SPLIT = 64;
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col, int per, int lanes) {
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int per, int lanes) {
     __shared__ float s_f[16 * MAX_SPLIT], s_l[16];
     __shared__ float4 s_p[256];
-    const int tid = threadIdx.x, lane = tid & 63, hd = a.hd;
-    const size_t col0 = (size_t)blockIdx.x * per;
-    const auto seq_of = [&](size_t col) { return (int)(col / a.cols / a.n_kv); };
-    for (int i = tid >> 6; i < per && col0 + i < n_col; i += 4) {
+    const int tid = threadIdx.x, lane = tid & 63, hd = a.hd, g = blockIdx.y, s = blockIdx.z, ns = a.splits[s];
+    const int c0 = blockIdx.x * per;
+    const size_t col0 = ((size_t)s * a.n_kv + g) * a.cols + c0;
+    for (int i = tid >> 6; i < per && c0 + i < a.cols; i += 4) {
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < a.splits[seq_of(col0 + i)]) ml = *(const float2 *)(a.part_ml + ((col0 + i) * a.n_split + lane) * 2);
+        if (lane < ns) ml = *(const float2 *)(a.part_ml + ((col0 + i) * a.n_split + lane) * 2);
         float C = ml.x;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) C = fmaxf(C, __shfl_xor(C, off));
@@ -290,12 +290,10 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col, in
     }
     __syncthreads();
     const int n_grp = 256 / (per * lanes), x = tid % lanes, grp = tid / lanes % n_grp, i = tid / (lanes * n_grp);
-    const size_t col = col0 + i;
-    const bool act = col < n_col && 4 * x < hd;
+    const bool act = c0 + i < a.cols && 4 * x < hd;
     float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
     if (act) {
-        const int ns = a.splits[seq_of(col)];
-        const float *o = a.part_o + col * a.n_split * hd + 4 * x;
+        const float *o = a.part_o + (col0 + i) * a.n_split * hd + 4 * x;
 #pragma unroll 8
         for (int p = grp; p < ns; p += n_grp) {
             const float f = s_f[i * MAX_SPLIT + p];
@@ -316,18 +314,19 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, size_t n_col, in
         r.z += v.z;
         r.w += v.w;
     }
-    const int c = (int)(col % a.cols), g = (int)(col / a.cols % a.n_kv), s = (int)(col / a.cols / a.n_kv);
-    store_out(a, s, g, c, 4 * x, r, 1.f / s_l[i]);
+    store_out(a, s, g, c0 + i, 4 * x, r, 1.f / s_l[i]);
 }
 
 // Many columns: a thread takes four dimensions of one, its splits eight at a
 // time (loads before their first use: a round trip to memory each time).
-__global__ __launch_bounds__(256) void k_tree_merge_flat(TreeArgs a, size_t n) {
-    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= n) return;
-    const int n4 = a.hd / 4, x = (int)(t % n4);
-    const size_t col = t / n4;
-    const int c = (int)(col % a.cols), g = (int)(col / a.cols % a.n_kv), s = (int)(col / a.cols / a.n_kv), ns = a.splits[s];
+// blockIdx.y: the KV head, blockIdx.z: the sequence (64-bit divisions of one
+// linear index took more time than the loads).
+__global__ __launch_bounds__(256) void k_tree_merge_flat(TreeArgs a) {
+    const unsigned t = blockIdx.x * 256 + threadIdx.x, n4 = (unsigned)a.hd / 4;
+    const int x = (int)(t % n4), c = (int)(t / n4), g = blockIdx.y, s = blockIdx.z;
+    if (c >= a.cols) return;
+    const size_t col = ((size_t)s * a.n_kv + g) * a.cols + c;
+    const int ns = a.splits[s];
     const float2 *ml = (const float2 *)(a.part_ml + col * a.n_split * 2);
     const float *o = a.part_o + col * a.n_split * a.hd + 4 * x;
     float C = -INFINITY, L = 0.f;
@@ -1060,6 +1059,7 @@ void pick_splits(TreeArgs &a, int step_keys, int want, int least) {
     for (int s = 0; s < a.d.n_seq; s++) all += steps[s] = ((long long)a.d.len[s] + a.d.rows + step_keys - 1) / step_keys;
     long long size = (all * a.n_kv * a.n_qg + want - 1) / want;
     if (size < least) size = least;
+    if (a.cols > 1 << 20) size = all;  // (many columns fill the chip: their splits' sums would be large)
     a.n_split = 1;
     for (int s = 0; s < a.d.n_seq; s++) {
         long long n = (steps[s] + size / 2) / size;
@@ -1102,7 +1102,7 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
     const size_t n = n_col * (a.hd / 4);
     if (a.n_split == 1 || a.arrived) return SCRY_OK;
     if (n >= (size_t)1 << 15) {
-        hipLaunchKernelGGL(k_tree_merge_flat, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, n);
+        hipLaunchKernelGGL(k_tree_merge_flat, dim3((a.cols * (a.hd / 4) + 255) / 256, a.n_kv, a.d.n_seq), dim3(256), 0, s, a);
         SCRY_HIP(hipGetLastError());
     } else {
         int lanes = 1;
@@ -1111,7 +1111,7 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
         int per = 256 / lanes;
         while (per > 1 && 256 / (per * lanes) * 2 <= a.n_split) per /= 2;
         if (per > 16) per = 16;
-        hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)((n_col + per - 1) / per)), dim3(256), 0, s, a, n_col, per, lanes);
+        hipLaunchKernelGGL(k_tree_merge, dim3((a.cols + per - 1) / per, a.n_kv, a.d.n_seq), dim3(256), 0, s, a, per, lanes);
         SCRY_HIP(hipGetLastError());
     }
     return SCRY_OK;
@@ -1186,7 +1186,7 @@ using namespace scry;
 extern "C" {
 
 int scry_hip_tree_attention(scry_buf q, const scry_buf *k_caches, const scry_buf *v_caches, int n_seq, const int32_t *len,
-                            int rows, const int32_t *parents, int n_q, int n_kv, int head_dim, float scale, scry_buf *out) {
+                            int rows, const int64_t *parents, int n_q, int n_kv, int head_dim, float scale, scry_buf *out) {
     API_LOCK;
     SCRY_REQUIRE_INIT();
     const char *what = "tree_attention";
@@ -1216,7 +1216,7 @@ int scry_hip_tree_attention(scry_buf q, const scry_buf *k_caches, const scry_buf
 }
 
 int scry_hip_kv8_tree_attention(scry_buf q, const scry_kv8 *caches, int n_seq, const int32_t *len, int rows,
-                                const int32_t *parents, int n_q, float scale, scry_buf *out) {
+                                const int64_t *parents, int n_q, float scale, scry_buf *out) {
     API_LOCK;
     SCRY_REQUIRE_INIT();
     const char *what = "kv8_tree_attention";

@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) void k_verify(VfArgs a, VfIn in, DraftBatch d)
 }
 
 // Checks, uploads, runs and waits: *res is the pinned result [n_seq][2 + rows].
-int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, const int32_t *counts, const int32_t *parents,
+int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, const int32_t *counts, const int64_t *parents,
            const double *u, int n_seq, int rows, int vocab, const int **res) {
     const bool tree = !q;
     if (vocab <= 0 || rows < 1) return set_error(SCRY_ERR_INVALID, "%s: vocabulary and rows must be > 0", what);
@@ -339,7 +339,7 @@ int scry_hip_verify_draft(scry_buf p, scry_buf q, const int64_t *tokens, const i
     return SCRY_OK;
 }
 
-int scry_hip_verify_tree(scry_buf p, const int64_t *tokens, const int32_t *parents, const double *u, int n_seq, int rows,
+int scry_hip_verify_tree(scry_buf p, const int64_t *tokens, const int64_t *parents, const double *u, int n_seq, int rows,
                          int vocab, int64_t *paths, int64_t *accepted, int64_t *token) {
     std::lock_guard<std::recursive_mutex> lock(api_mutex());
     SCRY_REQUIRE_INIT();

@@ -102,6 +102,9 @@ int scry_hip_buf_len(scry_buf b, size_t *n);
  * orders the two sides (scry_hip_synchronize, hipStreamSynchronize).  Take a
  * new view to write to a storage that a bf16-mode matmul has read. */
 int scry_hip_buf_dlpack(scry_buf b, void *wait_stream, int wait, void **managed);
+/* The destructor for a Python capsule "dltensor" around such a tensor: ends it
+ * unless a consumer has taken it (and renamed the capsule). */
+void scry_hip_dlpack_capsule_end(void *capsule);
 int scry_hip_free(scry_buf b);
 
 /* DeviceBackend::i8_from_vec (mod.rs:17-18, `quantize` feature) */
@@ -259,8 +262,8 @@ int scry_hip_reshape_from_heads(scry_buf x, int batch, int seq, int n_heads, int
  * No counterpart in the reference, which decodes one token of one sequence at
  * a time over an f32 cache (llama.rs:371-468, generate.rs:51-89).
  *
- * A batch is n_seq sequences (1 to 16) of `rows` drafted tokens each; all
- * arrays of ints are host arrays.  start / len [n_seq]: the context rows of
+ * A batch is n_seq sequences (1 to 16) of `rows` drafted tokens each; arrays of
+ * whole numbers are host arrays.  start / len [n_seq]: the context rows of
  * each sequence; its drafted row i lies at cache row len + i.  parents
  * [n_seq][rows], or null: row i follows row i - 1 (one new token, a drafted
  * chain, a chunk of a prompt; any number of rows).  With parents the rows are
@@ -275,7 +278,7 @@ int scry_hip_reshape_from_heads(scry_buf x, int batch, int seq, int n_heads, int
  * angles) at position start + depth, a row's depth being the number of its
  * ancestors.  q is also multiplied by q_scale; v is copied.  Outputs [n_seq *
  * rows, n_q * head_dim] and twice [n_seq * rows, n_kv * head_dim]. */
-int scry_hip_qk_norm_rope(scry_buf qkv, int n_seq, int rows, const int32_t *start, const int32_t *parents, int n_q,
+int scry_hip_qk_norm_rope(scry_buf qkv, int n_seq, int rows, const int32_t *start, const int64_t *parents, int n_q,
                           int n_kv, int head_dim, scry_buf freqs, scry_buf q_weight, scry_buf k_weight, float eps,
                           float q_scale, scry_buf *q, scry_buf *k, scry_buf *v);
 
@@ -303,9 +306,9 @@ int scry_hip_kv8_keep(const scry_kv8 *caches, int n_seq, const int32_t *start, c
  * Keys outside that set may hold anything.  The f32 form reads caches of rows
  * [n_kv * head_dim] (what scatter_rows fills), at least len + rows of them. */
 int scry_hip_tree_attention(scry_buf q, const scry_buf *k_caches, const scry_buf *v_caches, int n_seq, const int32_t *len,
-                            int rows, const int32_t *parents, int n_q, int n_kv, int head_dim, float scale, scry_buf *out);
+                            int rows, const int64_t *parents, int n_q, int n_kv, int head_dim, float scale, scry_buf *out);
 int scry_hip_kv8_tree_attention(scry_buf q, const scry_kv8 *caches, int n_seq, const int32_t *len, int rows,
-                                const int32_t *parents, int n_q, float scale, scry_buf *out);
+                                const int64_t *parents, int n_q, float scale, scry_buf *out);
 
 /* Verification of drafted tokens against the target's probabilities (rows of
  * softmax), with given random numbers u in [0, 1).  A draw from weights w with
@@ -327,7 +330,7 @@ int scry_hip_verify_draft(scry_buf p, scry_buf q, const int64_t *tokens, const i
  * row 0 the walk follows the child (the lowest) whose token is the drawn one.
  * paths [n_seq][rows]: the accepted nodes, then -1; accepted [n_seq]; token
  * [n_seq]: the token drawn from the last row. */
-int scry_hip_verify_tree(scry_buf p, const int64_t *tokens, const int32_t *parents, const double *u, int n_seq, int rows,
+int scry_hip_verify_tree(scry_buf p, const int64_t *tokens, const int64_t *parents, const double *u, int n_seq, int rows,
                          int vocab, int64_t *paths, int64_t *accepted, int64_t *token);
 
 /* ------------------------------------------------------ Llama (llama.rs) */

@@ -206,7 +206,7 @@ st("verify_draft", p2.h, p1.h, t1, None, None, 1, 1, 1, o1, o1)
 st("verify_draft", p2.h, None, t1, None, u1, 1, 1, 1, o1, o1)
 st("verify_draft", p2.h, p1.h, t1, None, u1, 1, 1, 1, None, o1)
 st("verify_tree", p2.h, t1, None, u1, 1, 1, 1, o1, o1, o1)
-st("verify_tree", p2.h, t1, (C.c_int32 * 1)(-1), u1, 1, 1, 1, None, o1, o1)
+st("verify_tree", p2.h, t1, (C.c_int64 * 1)(-1), u1, 1, 1, 1, None, o1, o1)
 """,
 }
 
