@@ -19,6 +19,7 @@ from ._lib import call, load
 _CAPSULE_NEW = C.pythonapi.PyCapsule_New
 _CAPSULE_NEW.restype, _CAPSULE_NEW.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
 _capsule_end = None  # the library's destructor of such capsules, on first use
+_device = 0  # the device of init_gpu
 
 
 def _f32(a) -> np.ndarray:
@@ -40,15 +41,17 @@ class Storage:
         return out
 
     def __dlpack_device__(self) -> tuple[int, int]:
-        return 10, 0  # ROCm; the library runs on one device (init)
+        return 10, _device  # ROCm
 
-    def __dlpack__(self, stream=None, **_):
+    def __dlpack__(self, *, stream=None, max_version=None, dl_device=None, copy=None):
         """The f32 values where they lie on the device, without a copy, for
         torch.from_dlpack and its like (torch imported before this package, so
         that both use one HIP runtime).  stream: what it does next comes after
         the ops called so far (None, 0, 1: the default stream); -1: the caller
         waits, as with HipBackend.synchronize().  Writes through the view, and
         reads that outlive it, are ordered by the caller."""
+        if copy or (dl_device is not None and tuple(dl_device) != self.__dlpack_device__()):
+            raise BufferError("a storage is viewed where it lies")
         global _capsule_end
         if _capsule_end is None:
             _capsule_end = C.cast(load().scry_hip_dlpack_capsule_end, C.c_void_p)
@@ -175,7 +178,9 @@ class HipBackend:
     # ---- runtime (cuda.rs:39-52 init_gpu, 1193-1197 synchronize)
     @staticmethod
     def init_gpu(device: int = 0) -> None:
+        global _device
         call("scry_hip_init", device)
+        _device = device
 
     @staticmethod
     def synchronize() -> None:
@@ -206,7 +211,9 @@ class HipBackend:
     @staticmethod
     def init_gpu_bf16(device: int = 0) -> None:
         """init_gpu_bf16 (cuda.rs:55-59): init, then bf16 mode."""
+        global _device
         call("scry_hip_init_bf16", device)
+        _device = device
 
     @staticmethod
     def set_bf16_mode(on: bool) -> None:

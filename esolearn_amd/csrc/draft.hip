@@ -35,8 +35,8 @@ int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, con
     b->rows = rows;
     b->tree = parents != nullptr;
     for (int s = 0; s < n_seq; s++) {
-        if (start[s] < 0 || start[s] > 0x7fffffff - rows)
-            return set_error(SCRY_ERR_RANGE, "%s: sequence %d starts at row %d", what, s, start[s]);
+        if (start[s] < 0 || start[s] > DRAFT_MAX_ROW - rows)  // (the kernels count rows in 32 bits, past the last by a step)
+            return set_error(SCRY_ERR_RANGE, "%s: rows %d .. of sequence %d (rows 0 .. 2^30)", what, start[s], s);
         b->len[s] = start[s];
         for (int i = 0; parents && i < rows; i++) {
             const int64_t p = parents[(size_t)s * rows + i];

@@ -457,6 +457,7 @@ int launch_attn_prefill(const PrefillAttn &a, int n_seq, const PrefillSeqs &t, i
 // draft.hip -- what the ops on drafted tokens share
 constexpr int DRAFT_MAX_TREE = 64;  // nodes of a tree: an ancestor set is one 64-bit mask
 constexpr int DRAFT_MAX_HD = 256;   // head sizes: multiples of 4 up to here
+constexpr int DRAFT_MAX_ROW = 1 << 30;
 struct DraftBatch {                 // passed to kernels by value
     int n_seq, rows, tree;          // tree: 0 = row i's parent is row i - 1
     int len[PF_MAX_SEQS];           // context rows of each sequence: row i lies at len + i

@@ -341,7 +341,7 @@ int scry_hip_kv8_new(int max_seq, int n_kv, int head_dim, scry_kv8 *out) {
     if (!out) return set_error(SCRY_ERR_INVALID, "kv8_new: null output handle");
     *out = nullptr;
     SCRY_TRY(check_heads("kv8_new", 0, n_kv, head_dim));
-    if (max_seq <= 0 || max_seq > 0x7fffffff - 64) return set_error(SCRY_ERR_INVALID, "kv8_new: max_seq %d", max_seq);
+    if (max_seq <= 0 || max_seq > DRAFT_MAX_ROW) return set_error(SCRY_ERR_INVALID, "kv8_new: max_seq %d (1 .. 2^30)", max_seq);
     DeviceScope dev;
     auto *c = new (std::nothrow) scry_kv8_s;
     if (!c) return set_error(SCRY_ERR_OOM, "host allocation failed");

@@ -1151,7 +1151,7 @@ int tree_run(const char *what, scry_buf q, const TreeArgs &t, bool i8, const F32
     if (q->n != n * t.n_q * t.hd) return set_error(SCRY_ERR_INVALID, "%s: shape mismatch", what);
     TreeArgs a = t;
     a.nrep = a.n_q / a.n_kv;
-    if ((size_t)a.d.rows * a.nrep > 0x7fffff00) return set_error(SCRY_ERR_UNSUPPORTED, "%s: %d rows", what, a.d.rows);
+    if ((size_t)a.d.rows * a.nrep > (size_t)1 << 30) return set_error(SCRY_ERR_UNSUPPORTED, "%s: %d rows", what, a.d.rows);
     a.cols = a.d.rows * a.nrep;
     DeviceScope dev;
     scry_buf o = nullptr;

@@ -49,6 +49,8 @@ refuse(INVALID, f, start=())
 refuse(INVALID, f, start=[0] * 17)
 refuse(RANGE, f, start=[-1])
 refuse(RANGE, f, start=[0x7fffffff])
+refuse(RANGE, f, start=[(1 << 30) - rows + 1])
+f(start=[(1 << 30) - rows])
 refuse(UNSUPPORTED, f, rows=65, parents=[-1] * 65)
 for bad in ([0, 0, 0, 0, 0], [-1, 1, 0, 0, 0], [-3, 0, 0, 0, 0], [-1, 0, -2, 2, 0], [-1, 0, 0, 0, 4]):
     refuse(INVALID, f, parents=bad)
@@ -63,6 +65,7 @@ with pytest.raises(ValueError):
     "kv8": """
 refuse(INVALID, B.kv8_new, 0, nkv, hd)
 refuse(INVALID, B.kv8_new, 0x7fffffff, nkv, hd)
+refuse(INVALID, B.kv8_new, (1 << 30) + 1, nkv, hd)
 refuse(INVALID, B.kv8_new, 10, 0, hd)
 refuse(UNSUPPORTED, B.kv8_new, 10, 1, 30)
 refuse(UNSUPPORTED, B.kv8_new, 10, 1, 512)

@@ -257,6 +257,71 @@ def test_attention(hip, cache, n_q, n_kv, hd, lens, rows, kind):
 
 
 @pytest.mark.parametrize("cache", ["f32", "int8"])
+@pytest.mark.parametrize("tiles", [1, 2, 3, 4, 5, 7])
+@pytest.mark.parametrize("hd", [16, 60, 64, 68, 128, 132, 192, 196, 256])
+def test_attention_every_shape_of_kernel(hip, cache, hd, tiles):
+    """Head sizes about the 64-dimension blocks, columns about the 16-column
+    tiles and groups of them, contexts that end in and at a step of keys."""
+    B = hip.HipBackend
+    n_q, n_kv = 2, 2
+    rows = 16 * tiles - 3
+    lens = [0, 63, 130, 64 * tiles - rows + 64]
+    kind = "tree" if rows <= 64 else "chain"
+    q, k, v, par = attention_case(n_q, n_kv, hd, lens, rows, kind, tiles)
+    scale = 1.0 / math.sqrt(hd)
+    pa = par if kind == "tree" else None
+    if cache == "f32":
+        o = B.tree_attention(B.from_vec(q), [B.from_vec(a) for a in k], [B.from_vec(b) for b in v], lens, rows, n_q, n_kv, hd,
+                             scale, parents=pa)
+    else:
+        caches = []
+        for a, b in zip(k, v):
+            caches.append(B.kv8_new(len(a), n_kv, hd))
+            B.kv8_write(caches[-1:], B.from_vec(a), B.from_vec(b), [0], len(a))
+        o = B.kv8_tree_attention(B.from_vec(q), caches, lens, rows, n_q, scale, parents=pa)
+        k, v = [stored(a) for a in k], [stored(b) for b in v]
+    ref, tol = attend(q, k, v, lens, par, float(F(scale)))
+    check_close(o.to_vec().reshape(q.shape), ref, tol)
+
+
+@pytest.mark.parametrize("cache", ["f32", "int8"])
+@pytest.mark.parametrize("n_q,n_kv,rows,ln", [(4, 1, 1, 20000), (2, 1, 20, 9000), (32, 1, 2, 6000), (64, 1, 16, 3000)])
+def test_attention_long_contexts_in_splits(hip, cache, n_q, n_kv, rows, ln):
+    """Key splits joined by the last workgroup, by groups of threads, by a thread
+    per column: one sharp row (its key early, late) and broad ones."""
+    B = hip.HipBackend
+    hd = 64
+    q, k, v, par = attention_case(n_q, n_kv, hd, [ln, ln // 3], rows, "chain", 5)
+    q[1, 0, 0] = k[1][7, 0] * F(3)
+    q[0, rows - 1, n_q - 1] = k[0][ln - 2, 0] * F(3)
+    scale = 0.125
+    if cache == "f32":
+        o = B.tree_attention(B.from_vec(q), [B.from_vec(a) for a in k], [B.from_vec(b) for b in v], [ln, ln // 3], rows, n_q, n_kv,
+                             hd, scale)
+    else:
+        caches = []
+        for a, b in zip(k, v):
+            caches.append(B.kv8_new(len(a), n_kv, hd))
+            B.kv8_write(caches[-1:], B.from_vec(a), B.from_vec(b), [0], len(a))
+        o = B.kv8_tree_attention(B.from_vec(q), caches, [ln, ln // 3], rows, n_q, scale)
+        k, v = [stored(a) for a in k], [stored(b) for b in v]
+    got = o.to_vec().reshape(q.shape)
+    for s, n in enumerate((ln, ln // 3)):
+        for i in range(rows):
+            keys = n + i + 1
+            sc = k[s][:keys, 0].astype(np.float64) @ q[s, i].astype(np.float64).T * scale  # [keys, n_q]
+            p = np.exp(sc - sc.max(0))
+            p /= p.sum(0)
+            ref = p.T @ v[s][:keys, 0].astype(np.float64)
+            # as attend(): a score's error, and the sums'; chunks of keys are summed
+            # apart and joined, so no sum has more than 2^10 terms in a row, and the
+            # weights' steps are at most 2^-23 of the largest
+            ds = (hd + 8) * U * scale * np.abs(q[s, i]).max() * np.abs(k[s][:keys, 0]).sum(-1).max() + 4 * U * np.abs(sc).max()
+            tol = (2 * ds + (4 * 1024 + 32) * U) * np.abs(v[s][:keys, 0]).max()
+            assert np.abs(got[s, i] - ref).max() <= tol, (s, i, np.abs(got[s, i] - ref).max(), tol)
+
+
+@pytest.mark.parametrize("cache", ["f32", "int8"])
 def test_attention_hides_what_is_masked(hip, cache):
     """NaN and infinities in rows that a node does not see leave it alone; in
     rows that it sees, they reach it. Values of the type's lowest and highest."""
@@ -605,6 +670,14 @@ ptr = t.data_ptr()
 a.free()  # the tensor still holds the values
 others = [B.zeros(1 << 20) for _ in range(4)]
 assert np.array_equal(t.cpu().numpy(), x * 2)
+assert others[0].__dlpack_device__() == (10, 0)
+for bad in (dict(copy=True), dict(dl_device=(1, 0))):
+    try:
+        others[0].__dlpack__(**bad)
+    except BufferError:
+        pass
+    else:
+        raise AssertionError(bad)
 c = others[0].__dlpack__(stream=-1)
 held = torch.from_dlpack(others[0]).data_ptr()
 del c, others
