@@ -29,6 +29,7 @@ namespace {
 using namespace dev;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -376,10 +377,11 @@ __device__ __forceinline__ void step_range(const TreeArgs &a, const Unit &u, int
 // its row's largest value in three balanced int8 digits, so the products and
 // their sums over hd are exact integers.
 // p.v: V's bytes become f16 (exact), and w = p * (the row's scale) is split
-// into two f16 terms, 22 bits.  c starts as max s + log2(the largest scale) - 8
-// and moves where a w passes 2^15: f16's smallest steps lie 2^-32 below the
-// largest w or further.  Scales below 2^-80 count as 2^-80 there, which keeps
-// 2^-c in f32's range.
+// into two f16 terms, each rounded to the nearest: 2^-24 of w, or where w is
+// small f16's smallest steps.  c starts as max s + log2(the largest scale) - 12
+// and moves where a w passes 2^15, so those steps lie 2^-36 below the largest w
+// or further.  Scales below 2^-80 count as 2^-80 there, which keeps 2^-c in f32's
+// range.
 // KS: steps of 64 dimensions (hdp <= 64 KS).
 
 // Column c's query as digits: lane (cl, j) holds dimensions 64 k + 16 j ..;
@@ -457,18 +459,17 @@ __device__ __forceinline__ void digit_scores(const i32x4 (&kk)[N][KS], const i32
 }
 
 // A column's running state: the reference c, the largest score and the
-// exponent of the largest scale - 8 when it last moved, the sum of the weights.
+// exponent of the largest scale - 12 when it last moved, the sum of the weights.
 struct RunI8 {
-    float c = -INFINITY, m = -INFINITY, ve = -88.f, l = 0.f;
+    float c = -INFINITY, m = -INFINITY, ve = -92.f, l = 0.f;
 };
 
 // Weights as two f16 terms, in the order of the operands of w.v.
 __device__ __forceinline__ void split_weights(const float (&w)[4], int x, f16x8 (&wh)[2], f16x8 (&wl)[2]) {
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
-        const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w[i], w[i + 1]));
-        const f16x2 lo = __builtin_bit_cast(
-            f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf(-(float)h[0], 1.f, w[i]), fmaf(-(float)h[1], 1.f, w[i + 1])));
+        const f16x2 h = __builtin_convertvector((f32x2{w[i], w[i + 1]}), f16x2);
+        const f16x2 lo = __builtin_convertvector((f32x2{fmaf(-(float)h[0], 1.f, w[i]), fmaf(-(float)h[1], 1.f, w[i + 1])}), f16x2);
         wh[x / 2][4 * (x % 2) + i] = h[0];
         wh[x / 2][4 * (x % 2) + i + 1] = h[1];
         wl[x / 2][4 * (x % 2) + i] = lo[0];
@@ -501,7 +502,7 @@ __device__ __forceinline__ float softmax_step(RunI8 &r, const f32x4 (&sc)[4], KQ
             split_weights(w, x, wh, wl);
         }
         // (a NaN weight makes the sum a NaN)
-        if (!__any(!(top <= 0x1p15f && sum <= 0x1p90f))) {
+        if (!__any(!(top <= 0x1p15f && sum <= 0x1p96f))) {
             r.l += sum;
             return 1.f;
         }
@@ -522,8 +523,8 @@ __device__ __forceinline__ float softmax_step(RunI8 &r, const f32x4 (&sc)[4], KQ
     }
     vm = col_max(vm);
     r.m = fmaxf(r.m, col_max(mx));
-    // 2^e >= the largest scale * 2^-8, e >= -88
-    r.ve = fmaxf(r.ve, (float)((int)((__float_as_uint(fmaxf(vm, 0x1p-80f)) + 0x7fffffu) >> 23) - 127 - 8));
+    // 2^e >= the largest scale * 2^-12, e >= -92
+    r.ve = fmaxf(r.ve, (float)((int)((__float_as_uint(fmaxf(vm, 0x1p-80f)) + 0x7fffffu) >> 23) - 127 - 12));
     // no score yet: a reference that the first one exceeds
     const float c = r.m == -INFINITY ? -INFINITY : r.m + r.ve, ref = c == -INFINITY ? 0.f : c;
     const float al = r.c == -INFINITY ? 0.f : exp2_fast(r.c - ref);
