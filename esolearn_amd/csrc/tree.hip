@@ -367,9 +367,9 @@ template <int SK>
 __device__ __forceinline__ void step_range(const TreeArgs &a, const Unit &u, int cols, int *lo, int *hi) {
     int rows = a.d.rows;
     if (!a.d.tree) rows = min(rows, (min(a.cols, (u.qg + 1) * cols) - 1) / a.nrep + 1);
-    const long long steps = ((long long)a.d.len[u.s] + rows + SK - 1) / SK;
-    *lo = (int)(steps * u.split / a.splits[u.s]);
-    *hi = (int)(steps * (u.split + 1) / a.splits[u.s]);
+    const unsigned steps = (unsigned)(a.d.len[u.s] + rows + SK - 1) / SK, ns = a.splits[u.s], each = steps / ns, more = steps % ns;
+    *lo = (int)(u.split * each + min((unsigned)u.split, more));
+    *hi = *lo + (int)(each + ((unsigned)u.split < more));
 }
 
 // ------------------------------------------------------------ int8 cache
@@ -392,7 +392,7 @@ __device__ __forceinline__ float query_digits(const TreeArgs &a, const Unit &u, 
     const float *q = a.q + (((size_t)u.s * a.d.rows + node) * a.n_q + u.g * a.nrep + rep) * hd;
     float4 x[KS][4];
     float m = 0.f;
-    bool fin = true;
+    bool nan = false;
 #pragma unroll
     for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -401,10 +401,10 @@ __device__ __forceinline__ float query_digits(const TreeArgs &a, const Unit &u, 
             x[k][e] = d < hd ? *(const float4 *)(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
             const float4 v = x[k][e];
             m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-            fin &= isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
+            nan |= __builtin_isunordered(v.x, v.y) || __builtin_isunordered(v.z, v.w);
         }
     // a query with an infinity or NaN has no finite softmax over any key
-    m = col_max(fin ? fmaxf(m, 0x1p-96f) : INFINITY);
+    m = col_max(nan ? INFINITY : fmaxf(m, 0x1p-96f));
     const float up = m < INFINITY ? 8290000.f / m : 0.f;  // 126.5 * 2^16: the top digit stays below 128
 #pragma unroll
     for (int k = 0; k < KS; k++)
