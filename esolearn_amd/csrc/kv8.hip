@@ -124,8 +124,10 @@ __device__ __forceinline__ float quantise(float4 x, int (&q)[4]) {
         q[i] = s > 0.f ? (int)copysignf(to_nearest(fabsf(v[i]), floorf(fabsf(v[i]) / s), s), v[i]) : 0;
     return s;
 }
+// the low bytes of four integers as a word
 __device__ __forceinline__ unsigned bytes4(int a, int b, int c, int d) {
-    return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)(d & 255) << 24;
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm((unsigned)d, (unsigned)c, 0x0c0c0400u),
+                                 __builtin_amdgcn_perm((unsigned)b, (unsigned)a, 0x0c0c0400u), 0x05040100u);
 }
 
 // A workgroup takes one 64-row block of one head, of K or of V (blockIdx.y), of
@@ -149,8 +151,9 @@ __device__ __forceinline__ bool block_of(const Kv8Rows &a, Block &b) {
 constexpr int V_LD = 17;  // words per dimension of a V block in LDS: 16, and one against bank conflicts
 
 // Bound by HBM (4 bytes read, 1 written).  V's 64-byte groups hold one
-// dimension of 64 rows: a whole block is turned through LDS (four rows of a
-// dimension are a word) and written in 16-byte pieces; part of a block in bytes.
+// dimension of 64 rows: four rows of a dimension are a word, words are turned
+// through LDS and written in 16-byte pieces (whole blocks) or one by one; the
+// rows about a word that is not the call's alone, in bytes.
 // 2047 rows of 32 heads of 128: 24 us, with V in bytes throughout 54 us.
 template <int G>
 __global__ __launch_bounds__(256) void k_kv8_write(Kv8Rows a, const float *__restrict__ kx, const float *__restrict__ vx) {
@@ -166,34 +169,8 @@ __global__ __launch_bounds__(256) void k_kv8_write(Kv8Rows a, const float *__res
     auto row = [&](int r) {
         return act ? *(const float4 *)(src + (b.src + (size_t)r * n_kv) * hd) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
-    if (b.v && b.lo == 0 && b.hi == 64) {
-        for (int w = grp; w < 16; w += NG) {  // rows 4 w ..
-            float4 x[4];
-            int q[4][4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = row(4 * w + i);
-            float sc[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) sc[i] = quantise<G>(x[i], q[i]);
-            if (gl == 0) *(float4 *)(scales + 4 * w) = make_float4(sc[0], sc[1], sc[2], sc[3]);
-            const int at = kv8_perm(4 * w) / 4;
-#pragma unroll
-            for (int e = 0; e < 4; e++) s_v[(4 * gl + e) * V_LD + at] = bytes4(q[0][e], q[1][e], q[2][e], q[3][e]) ^ 0x80808080u;
-        }
-        __syncthreads();
-        int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 0);
-        for (int t = tid; t < hd * 4; t += 256) {  // dimension t / 4, words 4 (t % 4) ..
-            const unsigned *w = s_v + (t >> 2) * V_LD + 4 * (t & 3);
-            *(uint4 *)(d + 16 * t) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        return;
-    }
-#pragma unroll 4
-    for (int r = b.lo + grp; r < b.hi; r += NG) {
-        int q[4];
-        const float sc = quantise<G>(row(r), q);
-        if (gl == 0) scales[r] = sc;
-        if (!act) continue;
+    auto put_row = [&](int r, const int (&q)[4]) {
+        if (!act) return;
         if (b.v) {
             int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 4 * gl) + kv8_perm(r);
 #pragma unroll
@@ -201,6 +178,52 @@ __global__ __launch_bounds__(256) void k_kv8_write(Kv8Rows a, const float *__res
         } else {
             *(unsigned *)(a.c.k[s] + kv8_k_at(rows_p, hdp, b.g, b.r0 + r) + 4 * gl) = bytes4(q[0], q[1], q[2], q[3]);
         }
+    };
+    constexpr int NQ = NG < 16 ? 16 / NG : 1;  // four rows at a time: rows 4 (grp + n NG) ..
+    float4 x[NQ][4];
+#pragma unroll
+    for (int n = 0; n < NQ; n++)  // every load before the first use
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 4 * (grp + n * NG) + i;
+            x[n][i] = r >= b.lo && r < b.hi ? row(r) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int r0 = 4 * (grp + n * NG);
+        if (r0 + 4 <= b.lo || r0 >= b.hi) continue;
+        int q[4][4];
+        float sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) sc[i] = quantise<G>(x[n][i], q[i]);
+        const bool whole = r0 >= b.lo && r0 + 4 <= b.hi;
+        if (whole && gl == 0) *(float4 *)(scales + r0) = make_float4(sc[0], sc[1], sc[2], sc[3]);
+        if (whole && b.v) {
+            const int at = kv8_perm(r0) / 4;
+#pragma unroll
+            for (int e = 0; e < 4; e++) s_v[(4 * gl + e) * V_LD + at] = bytes4(q[0][e], q[1][e], q[2][e], q[3][e]) ^ 0x80808080u;
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (r0 + i < b.lo || r0 + i >= b.hi) continue;
+            put_row(r0 + i, q[i]);
+            if (!whole && gl == 0) scales[r0 + i] = sc[i];
+        }
+    }
+    if (!b.v) return;
+    __syncthreads();
+    int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 0);
+    if (b.lo == 0 && b.hi == 64) {
+        for (int t = tid; t < hd * 4; t += 256) {  // dimension t / 4, words 4 (t % 4) ..
+            const unsigned *w = s_v + (t >> 2) * V_LD + 4 * (t & 3);
+            *(uint4 *)(d + 16 * t) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return;
+    }
+    for (int t = tid; t < hd * 16; t += 256) {  // word t % 16: rows 16 (t % 4) + 4 (t / 4 % 4) ..
+        const int r0 = 16 * (t & 3) + 4 * ((t >> 2) & 3);
+        if (r0 >= b.lo && r0 + 4 <= b.hi) *(unsigned *)(d + 4 * t) = s_v[(t >> 4) * V_LD + (t & 15)];
     }
 }
 
@@ -221,7 +244,7 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Rows a, float *__restrict__
             make_float4((float)(int)(signed char)(w0 >> sh) * sc, (float)(int)(signed char)(w1 >> sh) * sc,
                         (float)(int)(signed char)(w2 >> sh) * sc, (float)(int)(signed char)(w3 >> sh) * sc);
     };
-    if (b.v && b.lo == 0 && b.hi == 64) {
+    if (b.v) {
         const int8_t *d = a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 0);
         for (int t = tid; t < hd * 4; t += 256) {
             const uint4 x = *(const uint4 *)(d + 16 * t);
@@ -234,13 +257,14 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Rows a, float *__restrict__
         __syncthreads();
         if (!act) return;
         for (int w = grp; w < 16; w += NG) {
+            if (4 * w + 4 <= b.lo || 4 * w >= b.hi) continue;
             const unsigned *x = s_v + 4 * gl * V_LD + kv8_perm(4 * w) / 4;
             const float4 sc = *(const float4 *)(scales + 4 * w);
+            const float scs[4] = {sc.x, sc.y, sc.z, sc.w};
             const unsigned w0 = x[0], w1 = x[V_LD], w2 = x[2 * V_LD], w3 = x[3 * V_LD];
-            put(4 * w, w0, w1, w2, w3, 0, sc.x);
-            put(4 * w + 1, w0, w1, w2, w3, 8, sc.y);
-            put(4 * w + 2, w0, w1, w2, w3, 16, sc.z);
-            put(4 * w + 3, w0, w1, w2, w3, 24, sc.w);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (4 * w + i >= b.lo && 4 * w + i < b.hi) put(4 * w + i, w0, w1, w2, w3, 8 * i, scs[i]);
         }
         return;
     }
@@ -248,13 +272,8 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Rows a, float *__restrict__
 #pragma unroll 4
     for (int r = b.lo + grp; r < b.hi; r += NG) {
         const float sc = scales[r];
-        if (b.v) {
-            const uint8_t *d = (const uint8_t *)a.c.v[s] + kv8_v_at(rows_p, hdp, b.g, b.r0, 4 * gl) + kv8_perm(r);
-            put(r, d[0] ^ 0x80u, d[64] ^ 0x80u, d[128] ^ 0x80u, d[192] ^ 0x80u, 0, sc);
-        } else {
-            const unsigned w = *(const unsigned *)(a.c.k[s] + kv8_k_at(rows_p, hdp, b.g, b.r0 + r) + 4 * gl);
-            put(r, w, w >> 8, w >> 16, w >> 24, 0, sc);
-        }
+        const unsigned w = *(const unsigned *)(a.c.k[s] + kv8_k_at(rows_p, hdp, b.g, b.r0 + r) + 4 * gl);
+        put(r, w, w >> 8, w >> 16, w >> 24, 0, sc);
     }
 }
 
