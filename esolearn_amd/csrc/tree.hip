@@ -498,7 +498,7 @@ __device__ __forceinline__ float softmax_step(RunI8 &r, const f32x4 (&sc)[4], KQ
                 sum += p;
                 w[i] = p * v[i];
             }
-            top = fmaxf(fmaxf(top, fmaxf(w[0], w[1])), fmaxf(w[2], w[3]));
+            top = fmaxf(fmaxf(fmaxf(fmaxf(top, w[0]), w[1]), w[2]), w[3]);
             split_weights(w, x, wh, wl);
         }
         // (a NaN weight makes the sum a NaN)
@@ -674,20 +674,25 @@ __global__ __launch_bounds__(64 * W, (KS == 1 ? 4 : KS == 2 ? 3 : 2) - (W < 4 ? 
     int lo, hi;
     step_range<64>(a, u, 16 * W, &lo, &hi);
 
+    // A lane's offsets in a step's K and V.  Dimensions past hdp are taken from
+    // the last ones: they meet zero digits of q, or make outputs nobody stores.
     i32x4 kr[XB][KS], vr[DB];
+    int ko[XB][KS], vo[DB];
     float sr = 0.f;
+#pragma unroll
+    for (int b = 0; b < XB; b++)
+#pragma unroll
+        for (int k = 0; k < KS; k++) ko[b][k] = (16 * min(W * b + wave, 3) + cl) * hdp + min(64 * k + 16 * j, hdp - 16);
+#pragma unroll
+    for (int b = 0; b < DB; b++) vo[b] = min(16 * (W * b + wave) + cl, hdp - 1) * 64 + 16 * j;
     auto fetch = [&](int st) {
         const int8_t *kt = kb + (size_t)st * 64 * hdp, *vt = vb + (size_t)st * 64 * hdp;
 #pragma unroll
         for (int b = 0; b < XB; b++)
-            if (W * b + wave < 4)
 #pragma unroll
-                for (int k = 0; k < KS; k++)
-                    kr[b][k] = 64 * k + 16 * j < hdp ? *(const i32x4 *)(kt + (16 * (W * b + wave) + cl) * hdp + 64 * k + 16 * j)
-                                                     : i32x4{0, 0, 0, 0};
+            for (int k = 0; k < KS; k++) kr[b][k] = *(const i32x4 *)(kt + ko[b][k]);
 #pragma unroll
-        for (int b = 0; b < DB; b++)
-            vr[b] = 16 * (W * b + wave) < hdp ? *(const i32x4 *)(vt + (16 * (W * b + wave) + cl) * 64 + 16 * j) : i32x4{0, 0, 0, 0};
+        for (int b = 0; b < DB; b++) vr[b] = *(const i32x4 *)(vt + vo[b]);
         if (tid < 128) sr = scb[(size_t)st * 64];
     };
     if (lo < hi) fetch(lo);
@@ -696,12 +701,12 @@ __global__ __launch_bounds__(64 * W, (KS == 1 ? 4 : KS == 2 ? 3 : 2) - (W < 4 ? 
         __syncthreads();  // the step before has been read
 #pragma unroll
         for (int b = 0; b < XB; b++)
-            if (W * b + wave < 4)
+            if (W * b + W <= 4 || W * b + wave < 4)
 #pragma unroll
                 for (int k = 0; k < KS; k++) s_k[W * b + wave][k][lane] = kr[b][k];
 #pragma unroll
         for (int b = 0; b < DB; b++)
-            if (W * b + wave < DT) {
+            if (W * b + W <= DT || W * b + wave < DT) {
                 s_v[W * b + wave][0][lane] = v_operand(vr[b][0], vr[b][1]);
                 s_v[W * b + wave][1][lane] = v_operand(vr[b][2], vr[b][3]);
             }
@@ -959,17 +964,32 @@ __global__ __launch_bounds__(64 * W, ET <= 2 ? 3 : ET == 4 && W == 2 ? 1 : 2) vo
     int lo, hi;
     step_range<16 * KB>(a, u, 16 * W, &lo, &hi);
 
+    // Steps whose rows are all there, of heads that fill their 64-dimension
+    // blocks, take a lane's fixed offsets: the checks took 2% of the time.
     f32x4 kr[NB], vr[NB];
+    int ko[NB], vo[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const int at = min(W * b + wave, KB * CT - 1), y = at / CT, x = at % CT, i = x / ET, e = x % ET;
+        ko[b] = (16 * y + cl) * ldk + 16 * x + 4 * j;
+        vo[b] = (16 * y + 4 * j + i) * ldk + 64 * e + 4 * cl;
+    }
     auto fetch = [&](int st) {
         const float *kt = kb + (size_t)st * 16 * KB * ldk, *vt = vb + (size_t)st * 16 * KB * ldk;
         const int left = rows_end - st * 16 * KB;
+        if (left >= 16 * KB && hd == 64 * ET) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                kr[b] = *(const f32x4 *)(kt + ko[b]);
+                vr[b] = *(const f32x4 *)(vt + vo[b]);
+            }
+            return;
+        }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            const int y = (W * b + wave) / CT, x = (W * b + wave) % CT, i = x / ET, e = x % ET;
-            const int rk = 16 * y + cl, rv = 16 * y + 4 * j + i;
-            const bool in = W * b + wave < KB * CT;
-            kr[b] = in && rk < left && 16 * x + 4 * j < hd ? *(const f32x4 *)(kt + (size_t)rk * ldk + 16 * x + 4 * j) : zero;
-            vr[b] = in && rv < left && 64 * e + 4 * cl < hd ? *(const f32x4 *)(vt + (size_t)rv * ldk + 64 * e + 4 * cl) : zero;
+            const int at = min(W * b + wave, KB * CT - 1), y = at / CT, x = at % CT, i = x / ET, e = x % ET;
+            kr[b] = 16 * y + cl < left && 16 * x + 4 * j < hd ? *(const f32x4 *)(kt + ko[b]) : zero;
+            vr[b] = 16 * y + 4 * j + i < left && 64 * e + 4 * cl < hd ? *(const f32x4 *)(vt + vo[b]) : zero;
         }
     };
     if (lo < hi) fetch(lo);
@@ -991,7 +1011,7 @@ __global__ __launch_bounds__(64 * W, ET <= 2 ? 3 : ET == 4 && W == 2 ? 1 : 2) vo
         __syncthreads();  // the step before has been read
 #pragma unroll
         for (int b = 0; b < NB; b++)
-            if (W * b + wave < KB * CT) {
+            if (W * b + W <= KB * CT || W * b + wave < KB * CT) {
                 s_k[W * b + wave][lane] = kr[b];
                 s_v[W * b + wave][lane] = vr[b];
             }
