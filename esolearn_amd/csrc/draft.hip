@@ -66,7 +66,7 @@ int host_block(size_t bytes, void **p) {
         SCRY_HIP(hipStreamSynchronize(ctx().stream));
         host_free();
         const size_t want = (bytes + 4095) & ~(size_t)4095;
-        SCRY_HIP(hipHostMalloc(&g_host, want, hipHostMallocDefault));
+        SCRY_HIP(hipHostMalloc(&g_host, want, hipHostMallocCoherent));
         g_host_bytes = want;
     }
     *p = g_host;

@@ -466,8 +466,8 @@ struct DraftBatch {                 // passed to kernels by value
 // Checks start and parents (host, [n_seq] and [n_seq][rows] or null) and fills b.
 int draft_batch(const char *what, int n_seq, int rows, const int32_t *start, const int64_t *parents, DraftBatch *b);
 int check_heads(const char *what, int n_q, int n_kv, int head_dim);  // n_q = 0: no query heads
-// pinned host memory that the device reads and writes, `bytes` large, kept until shutdown; its users wait
-// for the stream before they return
+// pinned host memory, coherent with the device, `bytes` large, kept until shutdown; its users return when
+// the device has written what it will
 int host_block(size_t bytes, void **p);
 // arrival counters (arrive.h) of the launches on the context's stream, zero between them
 constexpr size_t DRAFT_COUNTERS = 16384;

@@ -20,6 +20,8 @@
 // A chain reads one row of p (and of q) of a sequence and is bound by the
 // latency of that sequence of steps; a tree reads its rows once, at the rate of
 // the memory.
+#include <atomic>
+#include <chrono>
 #include <cmath>
 #include <cstring>
 
@@ -47,7 +49,7 @@ struct VfArgs {
     double *part;       // [n_seq][R][2][n_sub]: sums of the weights and of p; R = rows + 1 (tree) or 1
     int *drawn;         // tree: [n_seq][rows + 1]
     unsigned *arrived;  // [n_seq][VF_MAX_ROWS + 2]: workgroups per row, rows per sequence; zero between launches
-    int *out;           // pinned, [n_seq][2 + rows]: accepted, next token, path
+    int *out;           // pinned, [n_seq][3 + rows]: done, accepted, next token, path
     const double *u;    // null: in the arguments, with the tokens
     const int *tok;
 };
@@ -157,26 +159,34 @@ __device__ __forceinline__ int vf_draw(const VfArgs &a, const VfRow &w, const do
     return max(j, 0);
 }
 
+// A result's value to host memory, past every cache of the device; and, by the
+// wave that wrote them, once those stores are complete, that the result is there.
+__device__ __forceinline__ void to_host(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
+__device__ __forceinline__ void vf_done(const VfArgs &a, int s) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if ((threadIdx.x & 63) == 0) to_host(a.out + s * (3 + a.rows), 1);
+}
+
 // From row 0 to the child that holds the row's token, a node per lane.
 __device__ __forceinline__ void vf_walk(const VfArgs &a, const VfIn &in, const DraftBatch &d, int s) {
     const int i = threadIdx.x & 63;
     const int parent = i < a.rows ? (int)d.parent[s][i] : -2;
     const int tok = i < a.rows ? vf_tok(a, in)[s * (a.rows + 1) + i] : 0;
     const int t_row = i < a.rows ? get(a.drawn + s * (a.rows + 1) + 1 + i) : 0;  // drawn after node i
-    int *out = a.out + s * (2 + a.rows);
+    int *out = a.out + s * (3 + a.rows) + 1;
     int cur = -1, n = 0, t = get(a.drawn + s * (a.rows + 1));
     for (;;) {
         const unsigned long long hit = __ballot(parent == cur && tok == t);
         if (!hit) break;
         cur = __ffsll((long long)hit) - 1;  // above the last one: at most `rows` turns
-        if (i == 0) out[2 + n] = cur;
+        if (i == 0) to_host(out + 2 + n, cur);
         t = __shfl(t_row, cur);
         n++;
     }
-    if (i >= n && i < a.rows) out[2 + i] = -1;
+    if (i >= n && i < a.rows) to_host(out + 2 + i, -1);
     if (i == 0) {
-        out[0] = n;
-        out[1] = t;
+        to_host(out, n);
+        to_host(out + 1, t);
     }
 }
 
@@ -221,16 +231,19 @@ __global__ __launch_bounds__(256) void k_verify(VfArgs a, VfIn in, DraftBatch d)
             if (a.tree) {
                 put(a.drawn + s * (a.rows + 1) + r, j);
             } else {
-                a.out[s * (2 + a.rows)] = w.n;
-                a.out[s * (2 + a.rows) + 1] = j;
+                to_host(a.out + s * (3 + a.rows) + 1, w.n);
+                to_host(a.out + s * (3 + a.rows) + 2, j);
             }
         }
+        if (!a.tree) vf_done(a, s);
     }
     if (!a.tree || !last_to_arrive(arrived, gridDim.y)) return;
-    if (wave == 0) vf_walk(a, in, d, s);
+    if (wave != 0) return;
+    vf_walk(a, in, d, s);
+    vf_done(a, s);
 }
 
-// Checks, uploads, runs and waits: *res is the pinned result [n_seq][2 + rows].
+// Checks, uploads, runs and waits: *res is the pinned result [n_seq][3 + rows].
 int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, const int32_t *counts, const int64_t *parents,
            const double *u, int n_seq, int rows, int vocab, const int **res) {
     const bool tree = !q;
@@ -283,11 +296,12 @@ int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, cons
         }
     }
     const bool big = n > VF_ARGS;
-    const size_t out_bytes = (n_seq * (m + 2) * sizeof(int) + 255) & ~(size_t)255;
+    const size_t out_bytes = (n_seq * (m + 3) * sizeof(int) + 255) & ~(size_t)255;
     DeviceScope dev;
     char *host = nullptr;
     SCRY_TRY(host_block(out_bytes + n * (sizeof(double) + sizeof(int)), (void **)&host));
     a.out = (int *)host;
+    for (int s = 0; s < n_seq; s++) a.out[s * (m + 3)] = 0;  // (no launch writes them any more)
     std::memcpy(big ? (double *)(host + out_bytes) : in.u, hu, n * sizeof(double));
     std::memcpy(big ? (int *)(host + out_bytes + n * sizeof(double)) : in.tok, ht, n * sizeof(int));
 
@@ -307,10 +321,26 @@ int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, cons
     }
     hipLaunchKernelGGL(k_verify, dim3((a.n_sub + 3) / 4, R, n_seq), dim3(256), 0, st, a, in, d);
     hipError_t e = hipGetLastError();
-    // the pinned block is read and written until here, whatever happened
-    const hipError_t w = hipStreamSynchronize(st);
-    if (e == hipSuccess) e = w;
-    if (e != hipSuccess) return hip_fail(e, what, __FILE__, __LINE__);
+    // The results are there when every sequence is done: the host looks for that
+    // for a while, which is 4 us sooner than the stream's own end is known (one chain
+    // at V = 32000 22.5 -> 18.3 us), and behind longer work, or where a result does
+    // not come, waits for the stream, which says why.
+    const volatile int *flag = a.out;
+    auto done = [&] {
+        for (int s = 0; s < n_seq; s++)
+            if (!flag[s * (m + 3)]) return false;
+        return true;
+    };
+    const auto until = std::chrono::steady_clock::now() + std::chrono::milliseconds(20);
+    bool seen = false;
+    while (e == hipSuccess && !(seen = done()) && std::chrono::steady_clock::now() < until) {
+    }
+    std::atomic_thread_fence(std::memory_order_acquire);
+    if (!seen) {
+        const hipError_t w = hipStreamSynchronize(st);
+        if (e == hipSuccess) e = w;
+        if (e != hipSuccess) return hip_fail(e, what, __FILE__, __LINE__);
+    }
     *res = a.out;
     return SCRY_OK;
 }
@@ -333,8 +363,8 @@ int scry_hip_verify_draft(scry_buf p, scry_buf q, const int64_t *tokens, const i
     const int *r = nullptr;
     SCRY_TRY(vf_run(what, p, q, tokens, counts, nullptr, u, n_seq, rows, vocab, &r));
     for (int s = 0; s < n_seq; s++) {
-        accepted[s] = r[(size_t)s * (rows + 2)];
-        token[s] = r[(size_t)s * (rows + 2) + 1];
+        accepted[s] = r[(size_t)s * (rows + 3) + 1];
+        token[s] = r[(size_t)s * (rows + 3) + 2];
     }
     return SCRY_OK;
 }
@@ -350,7 +380,7 @@ int scry_hip_verify_tree(scry_buf p, const int64_t *tokens, const int64_t *paren
     const int *r = nullptr;
     SCRY_TRY(vf_run(what, p, nullptr, tokens, nullptr, parents, u, n_seq, rows, vocab, &r));
     for (int s = 0; s < n_seq; s++) {
-        const int *x = r + (size_t)s * (rows + 2);
+        const int *x = r + (size_t)s * (rows + 3) + 1;
         accepted[s] = x[0];
         token[s] = x[1];
         for (int i = 0; i < rows; i++) paths[(size_t)s * rows + i] = x[2 + i];

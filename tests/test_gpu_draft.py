@@ -546,6 +546,25 @@ def test_verify_tree(hip, V, n_seq, rows):
         assert list(paths[s, :n[s]]) == want and (paths[s, n[s]:] == -1).all() and t[s] == x, s
 
 
+def test_verify_behind_queued_work(hip):
+    """Tens of milliseconds of other ops are queued before the call: it waits
+    for them, and its results are its own."""
+    B = hip.HipBackend
+    rng = np.random.default_rng(4)
+    V = 4000
+    a = B.from_vec(rng.normal(0, 1, 4096 * 4096).astype(F))
+    for turn in range(3):
+        p = softmax(rng.normal(0, 2, (2, 4, V)))
+        q = softmax(rng.normal(0, 2, (2, 3, V)))
+        tok, u = q.argmax(-1), rng.random((2, 4))
+        hp, hq = B.from_vec(p), B.from_vec(q)
+        held = [B.matmul(a, a, 4096, 4096, 4096) for _ in range(40 if turn else 1)]
+        n, t = B.verify_draft(hp, hq, tok, u, V)
+        for s in range(2):
+            assert (int(n[s]), int(t[s])) == draft_ref(p[s], q[s], tok[s], u[s], 3)
+        del held
+
+
 # ---------------------------------------------------------------- as they are used
 @pytest.mark.parametrize("cache", ["f32", "int8"])
 def test_a_speculative_run(hip, cache):
