@@ -116,6 +116,8 @@ struct QkArgs {
 // row (few rows: a part of its heads), so its hd/2 angles, the expensive f64
 // part, are computed once and lie in LDS; G lanes hold a head, a float4 each.
 // The sum of squares of a head is an f32 tree over its lanes.
+// 2047 rows of 96 heads of 128, 201 MB: 40 us, a large copy's rate; one row of
+// 48: 3.6 us.
 template <int G>
 __global__ __launch_bounds__(256) void k_qk_norm_rope(QkArgs a) {
     constexpr int NG = 256 / G;

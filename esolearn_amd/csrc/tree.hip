@@ -10,9 +10,11 @@
 // lane holds the scores of one column for 4 keys of each 16: the running
 // maximum and sum are lane values joined over 4 lanes, and the weights are
 // already the operand that the products p.v take, without a pass through LDS.
-// A wave takes QT tiles and every fourth step of keys; the four waves of a
-// workgroup are joined through LDS, and where the keys are split over
-// workgroups too, by k_tree_merge.
+// Few columns (narrow kernels): a workgroup has one tile, each of its four waves
+// every fourth step of keys, and they are joined through LDS.  Many (wide): a
+// wave has a tile, and the workgroup's tiles share each step's keys through LDS.
+// Where the keys are split over workgroups too, the last of them or k_tree_merge*
+// joins the splits.
 //
 // Workgroups go to the XCDs round-robin: those of one (sequence, KV head,
 // split) share their keys and sit on one XCD, so the keys come from its L2
@@ -559,7 +561,8 @@ __device__ __forceinline__ f16x8 v_operand(int w0, int w1) {
 }
 
 // Few columns (one tile a workgroup): bound by reading the cache.  Keys go
-// from memory to the operands, every wave with steps of its own.
+// from memory to the operands, every wave with steps of its own.  One token of
+// 32 heads (8 of K and V, 128 dimensions) over 65001 rows: 137 MB in 28.7 us.
 template <int KS>
 __global__ __launch_bounds__(64 * WAVES, KS <= 2 ? 2 : 1) void k_tree_i8(TreeArgs a, Kv8Batch cb) {
     constexpr int DT = 4 * KS, COLS = 16;
@@ -647,6 +650,8 @@ __global__ __launch_bounds__(64 * WAVES, KS <= 2 ? 2 : 1) void k_tree_i8(TreeArg
 // W waves with a tile each share the keys through LDS: each stages a part of
 // a step, V as f16 (converted once for the W tiles), in the order in which the
 // lanes take their operands, and holds the next step's part in registers.
+// 64-node trees of eight 4000-row contexts, 32 heads over 8 of 128: 26 GFLOP (65
+// in digits and terms) in 74 us.
 template <int KS, int W>
 __global__ __launch_bounds__(64 * W, (KS == 1 ? 4 : KS == 2 ? 3 : 2) - (W < 4 ? 1 : 0)) void k_tree_i8_wide(TreeArgs a, Kv8Batch cb) {
     constexpr int DT = 4 * KS, XB = (4 + W - 1) / W, DB = (DT + W - 1) / W;
@@ -933,6 +938,7 @@ __global__ __launch_bounds__(64 * WAVES, ET <= 3 ? 2 : 1) void k_tree_f32(TreeAr
 // a step's keys through LDS, in operand order; the next step's part waits in
 // registers.  A step is 16 keys, 32 where heads are short (at 128 dimensions 32
 // keys a step left fewer waves: 26-node trees of four contexts 62 against 56 us).
+// Those trees over 2047 rows, 32 heads over 8 of 128: 2.8 GFLOP in 47 us.
 constexpr int tree_f32_blocks(int et) { return et == 1 ? 2 : 1; }
 template <int ET, int W>
 __global__ __launch_bounds__(64 * W, ET <= 2 ? 3 : ET == 4 && W == 2 ? 1 : 2) void k_tree_f32_wide(TreeArgs a, F32Batch fb) {
@@ -1107,12 +1113,15 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
     const size_t grid = (size_t)((a.pair0[a.d.n_seq] + 7) / 8) * 8 * a.n_qg;
     if (grid > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "attention: %zu workgroups", grid);
     // Few splits of few columns: the last to arrive joins them, without a second
-    // launch (one token, 4 query heads a KV head, over 2000 rows: 15.9 -> 12.7
-    // us).  The wide kernels' columns are joined by a launch of their own, which
-    // has more workgroups for it (trees of eight 4000-row contexts: 79 us against
-    // 88 us joined by the last).
+    // launch (one token of 4 query heads a KV head over 2000 int8 rows: 14.8 ->
+    // 12.7 us).  From 2 MB of partial sums on, a launch of its own has more
+    // workgroups for them (16 rows of 32 heads of 128: over 4000 int8 rows, 2 MB,
+    // 18.5 us joined by the last and 19.0 by a launch, over 6000, 3 MB, 24.7 and
+    // 22.0), and so for the wide kernels' columns.
     a.arrived = nullptr;
-    if (a.n_split > 1 && a.n_split <= fused && (size_t)a.d.n_seq * a.n_kv * a.n_qg <= DRAFT_COUNTERS) SCRY_TRY(draft_counters(&a.arrived));
+    if (a.n_split > 1 && a.n_split <= fused && n_col * a.n_split * a.hd <= (size_t)1 << 19 &&
+        (size_t)a.d.n_seq * a.n_kv * a.n_qg <= DRAFT_COUNTERS)
+        SCRY_TRY(draft_counters(&a.arrived));
     if (lds > 65536)
         SCRY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * waves), lds, s, a, b);
@@ -1140,15 +1149,15 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
 
 // Workgroups that a launch aims at: three of four waves a CU (what the wide
 // int8 kernel's registers allow at 128 dimensions: 64-node trees of eight
-// 4000-row contexts 97 us at two, 79 at three, 97 at four, of which some wait).
-// The f32 kernels: 26-node trees of four 2047-row contexts 57.7 us at two, 56.1
-// at three, 66.9 at four.
+// 4000-row contexts 83 us at two, 73 at three, 75 at four, of which some wait;
+// a 512-row chunk over 1500 rows of 32 heads 56, 53 and 62).  The f32 kernels:
+// 26-node trees of four 2047-row contexts 51 us at two, 50 at three, 52 at four.
 constexpr int WANT = 768;
 constexpr int FUSED = 16;  // key splits that the last of a narrow kernel's workgroups joins
 
 // Columns in tiles of 16: three or four tiles share the keys (W waves).  One tile,
 // over int8 caches two, have the narrow kernel (8-node trees of 32 columns over
-// 2000 rows of four sequences: int8 23.4 us wide, 17.6 narrow, f32 35.2 and 39.7).
+// 2000 rows of four sequences: int8 19.4 us wide, 17.3 narrow, f32 32.6 and 40.0).
 template <int KS>
 int launch_i8(const TreeArgs &a, const Kv8Batch &b, hipStream_t s) {
     const int tiles = (a.cols + 15) / 16, groups = (tiles + 3) / 4, w = (tiles + groups - 1) / groups;

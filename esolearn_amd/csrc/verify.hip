@@ -18,8 +18,9 @@
 // leave the sums of their parts; the last workgroup of a row to arrive finds
 // the part, and in it the token; for a tree, the last row of a sequence walks.
 // A chain reads one row of p (and of q) of a sequence and is bound by the
-// latency of that sequence of steps; a tree reads its rows once, at the rate of
-// the memory.
+// latency of that sequence of steps (V = 32000: 9 us, 16 chains at 128256: 13);
+// a tree reads its rows once, at the rate of the memory, before the draws (four
+// trees of 31 nodes at V = 128256, 66 MB: 27 us).
 #include <atomic>
 #include <chrono>
 #include <cmath>
@@ -265,8 +266,10 @@ int vf_run(const char *what, scry_buf p, scry_buf q, const int64_t *tokens, cons
     a.tree = tree;
     a.wide = V % 4 == 0;
     const int R = tree ? rows + 1 : 1;
-    // a wave's part: 512 values (8 a lane), more where that gives more
-    // workgroups than the chip runs at once
+    // a wave's part: 512 values (8 a lane; 16 chains at V = 128256 22 us a call, 25
+    // at 256 values, 24 at 1024), more where that gives more workgroups than the
+    // chip runs at once (four trees of 31 nodes 38 us; 42 at half as many workgroups
+    // or twice as many)
     size_t sub = 512;
     while (sub < 4096 && (V + 4 * sub - 1) / (4 * sub) * R * n_seq > 2048) sub *= 2;
     a.sub = (int)sub;
