@@ -192,7 +192,7 @@ extern "C" int scry_hip_qk_norm_rope(scry_buf qkv, int n_seq, int rows, const in
     DraftBatch b;
     SCRY_TRY(draft_batch(what, n_seq, rows, start, parents, &b));
     const size_t n_rows = (size_t)n_seq * rows, hd = head_dim;
-    if (n_rows > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "%s: %zu rows", what, n_rows);
+    if (n_rows > DRAFT_MAX_GRID) return set_error(SCRY_ERR_UNSUPPORTED, "%s: %zu rows", what, n_rows);
     if (qkv->n != n_rows * (n_q + 2 * (size_t)n_kv) * hd || freqs->n != hd / 2 || (q_weight && q_weight->n != hd) ||
         (k_weight && k_weight->n != hd))
         return set_error(SCRY_ERR_INVALID, "%s: shape mismatch", what);

@@ -458,6 +458,7 @@ int launch_attn_prefill(const PrefillAttn &a, int n_seq, const PrefillSeqs &t, i
 constexpr int DRAFT_MAX_TREE = 64;  // nodes of a tree: an ancestor set is one 64-bit mask
 constexpr int DRAFT_MAX_HD = 256;   // head sizes: multiples of 4 up to here
 constexpr int DRAFT_MAX_ROW = 1 << 30;
+constexpr size_t DRAFT_MAX_GRID = 0xffffff;  // workgroups of 256 threads along x: a launch counts threads in 32 bits
 struct DraftBatch {                 // passed to kernels by value
     int n_seq, rows, tree;          // tree: 0 = row i's parent is row i - 1
     int len[PF_MAX_SEQS];           // context rows of each sequence: row i lies at len + i

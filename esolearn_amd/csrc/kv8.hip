@@ -340,7 +340,7 @@ int kv8_rows(const char *what, const scry_kv8 *caches, int n_seq, const int32_t 
         blocks = blocks > n ? blocks : n;
     }
     a->rows = rows;
-    if (blocks * a->c.n_kv > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what, rows, a->c.n_kv);
+    if (blocks * a->c.n_kv > DRAFT_MAX_GRID) return set_error(SCRY_ERR_UNSUPPORTED, "%s: %d rows of %d heads", what, rows, a->c.n_kv);
     *grid = dim3((unsigned)(blocks * a->c.n_kv), 2, n_seq);
     return SCRY_OK;
 }

@@ -1111,7 +1111,7 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
         a.pair0[i + 1] = a.pair0[i] + a.n_kv * a.splits[i];
     }
     const size_t grid = (size_t)((a.pair0[a.d.n_seq] + 7) / 8) * 8 * a.n_qg;
-    if (grid > 0x7fffffff) return set_error(SCRY_ERR_UNSUPPORTED, "attention: %zu workgroups", grid);
+    if (grid > DRAFT_MAX_GRID) return set_error(SCRY_ERR_UNSUPPORTED, "attention: %zu workgroups", grid);
     // Few splits of few columns: the last to arrive joins them, without a second
     // launch (one token of 4 query heads a KV head over 2000 int8 rows: 14.8 ->
     // 12.7 us).  From 2 MB of partial sums on, a launch of its own has more

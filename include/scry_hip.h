@@ -269,7 +269,8 @@ int scry_hip_reshape_from_heads(scry_buf x, int batch, int seq, int n_heads, int
  * chain, a chunk of a prompt; any number of rows).  With parents the rows are
  * a tree (at most 64): an earlier row, -1: the context, -2: no node (what pads
  * a smaller tree; its row of an attention is zero, and no node's parent).
- * head_dim: a multiple of 4, at most 256; start + rows at most 2^30. */
+ * head_dim: a multiple of 4, at most 256; start + rows at most 2^30; fewer than
+ * 2^24 rows, or (KV head, 64 rows) blocks, a call. */
 
 /* Per-head RMSNorm of q and k, and RoPE, in one pass over the fused qkv rows
  * [n_seq * rows, (n_q + 2 n_kv) * head_dim]: n = h / sqrt(mean(h^2) + eps) *

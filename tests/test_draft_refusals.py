@@ -51,6 +51,8 @@ refuse(RANGE, f, start=[-1])
 refuse(RANGE, f, start=[0x7fffffff])
 refuse(RANGE, f, start=[(1 << 30) - rows + 1])
 f(start=[(1 << 30) - rows])
+refuse(UNSUPPORTED, f, rows=1 << 24)
+refuse(UNSUPPORTED, f, start=[0] * 16, rows=1 << 20)
 refuse(UNSUPPORTED, f, rows=65, parents=[-1] * 65)
 for bad in ([0, 0, 0, 0, 0], [-1, 1, 0, 0, 0], [-3, 0, 0, 0, 0], [-1, 0, -2, 2, 0], [-1, 0, 0, 0, 4]):
     refuse(INVALID, f, parents=bad)
