@@ -321,6 +321,61 @@ def test_attention_long_contexts_in_splits(hip, cache, n_q, n_kv, rows, ln):
             assert np.abs(got[s, i] - ref).max() <= tol, (s, i, np.abs(got[s, i] - ref).max(), tol)
 
 
+@pytest.mark.parametrize("n_seq", [1, 2])
+@pytest.mark.parametrize("cache,ln", [("f32", 2000), ("int8", 4000)])
+def test_attention_of_many_heads_in_few_splits(hip, cache, ln, n_seq):
+    """One tile of columns of each of 40 KV heads, whose 16 (8) splits have more
+    partial sums than the last workgroup of a head joins."""
+    B = hip.HipBackend
+    n_kv, hd, rows = 40, 128, 16
+    lens = [ln, ln - 65][:n_seq]
+    q, k, v, par = attention_case(n_kv, n_kv, hd, lens, rows, "chain", 6)
+    scale = hd ** -0.5
+    if cache == "f32":
+        o = B.tree_attention(B.from_vec(q), [B.from_vec(a) for a in k], [B.from_vec(b) for b in v], lens, rows, n_kv, n_kv, hd, scale)
+    else:
+        caches = []
+        for a, b in zip(k, v):
+            caches.append(B.kv8_new(len(a), n_kv, hd))
+            B.kv8_write(caches[-1:], B.from_vec(a), B.from_vec(b), [0], len(a))
+        o = B.kv8_tree_attention(B.from_vec(q), caches, lens, rows, n_kv, scale)
+        k, v = [stored(a) for a in k], [stored(b) for b in v]
+    got = o.to_vec().reshape(q.shape)
+    for s, n in enumerate(lens):
+        seen = np.arange(n + rows)[:, None] <= n + np.arange(rows)  # [keys, rows]
+        for h in range(n_kv):
+            kk, vv = k[s][:, h].astype(np.float64), v[s][:, h].astype(np.float64)
+            sc = np.where(seen, kk @ q[s, :, h].astype(np.float64).T * scale, -np.inf)
+            p = np.exp(sc - sc.max(0))
+            ref = (p / p.sum(0)).T @ vv
+            # as in the long contexts above
+            ds = (hd + 8) * U * scale * np.abs(q[s, :, h]).max(-1) * np.abs(kk).sum(-1).max() + 4 * U * np.abs(np.where(seen, sc, 0)).max(0)
+            tol = (2 * ds + (4 * 1024 + 32) * U) * np.abs(vv).max()
+            assert (np.abs(got[s, :, h] - ref).max(-1) <= tol).all(), (s, h)
+
+
+@pytest.mark.parametrize("rows", [3, 30])
+@pytest.mark.parametrize("cache", ["f32", "int8"])
+def test_attention_scales_of_zero_and_below(hip, cache, rows):
+    """Scale 0: equal weights; a negative scale: the queries turned round."""
+    B = hip.HipBackend
+    n_q, n_kv, hd, lens = 8, 2, 64, [70, 0]
+    q, k, v, par = attention_case(n_q, n_kv, hd, lens, rows, "tree", 8)
+    if cache == "f32":
+        sk, sv = [B.from_vec(a) for a in k], [B.from_vec(b) for b in v]
+    else:
+        caches = []
+        for a, b in zip(k, v):
+            caches.append(B.kv8_new(len(a), n_kv, hd))
+            B.kv8_write(caches[-1:], B.from_vec(a), B.from_vec(b), [0], len(a))
+        k, v = [stored(a) for a in k], [stored(b) for b in v]
+    for scale in (0.0, -0.2):
+        x = B.from_vec(q)
+        o = B.tree_attention(x, sk, sv, lens, rows, n_q, n_kv, hd, scale, parents=par) if cache == "f32" else \
+            B.kv8_tree_attention(x, caches, lens, rows, n_q, scale, parents=par)
+        check_close(o.to_vec().reshape(q.shape), *attend(-q, k, v, lens, par, -scale))
+
+
 @pytest.mark.parametrize("cache", ["f32", "int8"])
 def test_attention_hides_what_is_masked(hip, cache):
     """NaN and infinities in rows that a node does not see leave it alone; in
