@@ -1164,8 +1164,8 @@ int launch_tree(K kernel, TreeArgs a, const B &b, int waves, int cols, size_t ld
 
 // Workgroups that a launch aims at: three of four waves a CU (what the wide
 // int8 kernel's registers allow at 128 dimensions: 64-node trees of eight
-// 4000-row contexts 83 us at two, 73 at three, 75 at four, of which some wait;
-// a 512-row chunk over 1500 rows of 32 heads 56, 53 and 62).  The f32 kernels:
+// 4000-row contexts 84 us at two, 75 at three, 76 at four, of which some wait;
+// a 512-row chunk over 1500 rows of 32 heads 50, 50 and 56).  The f32 kernels:
 // 26-node trees of four 2047-row contexts 51 us at two, 50 at three, 52 at four.
 constexpr int WANT = 768;
 constexpr int FUSED = 16;  // key splits that the last of a narrow kernel's workgroups joins
